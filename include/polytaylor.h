@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define PT_ABI_VERSION 15
+#define PT_ABI_VERSION 16
 #define PT_MAX_DEGREE 8
 /* Largest degree of the elementwise kernels (pt_activation_series_*, pt_series_binary): their
  * register plans are per element, so they run above PT_MAX_DEGREE. */
@@ -518,6 +518,98 @@ typedef enum pt_binary {
 int pt_series_binary(int dtype, int degree, int op, const void* const* a,
                      const void* const* b, void* const* y, int64_t numel,
                      void* stream);
+
+/*
+ * Dropout of `orders` (1..17) buffers of `numel` elements of `dtype` with one mask:
+ *   y_k[i] = keep(i) ? x_k[i] / (1 - p) : 0.
+ * keep(i): word i mod 4 of Philox4x32-10 at the counter (i / 4) under the key *seed (a device
+ * int64) is at least p 2^32. p in [0, 1]. The same call on a cotangent is the gradient.
+ * (The reference's rule for torch's dropout stores the mask:
+ *   /root/reference/src/polytensors/_dispatch.py.)
+ */
+int pt_dropout_series(int dtype, int orders, const void* const* x, void* const* y, int64_t numel, double p,
+                      const int64_t* seed, void* stream);
+
+/* Largest head of pt_norm_rope_series_*. */
+#define PT_NORM_ROPE_MAX_HEAD 256
+
+/*
+ * One operand (queries or keys) of pt_norm_rope_series_*: `heads` heads of head_dim elements for each
+ * of batch x length tokens. Pointer arrays are host arrays; those of the other direction are ignored.
+ */
+typedef struct pt_norm_rope_operand {
+  const void* const* x;      /* degree + 1 pointers: head h of token (b, l) starts at element */
+  int64_t stride_b;          /*   b stride_b + l stride_l + h stride_h, its elements side by side */
+  int64_t stride_l;
+  int64_t stride_h;
+  int64_t heads;
+  const void* const* weight; /* weight_orders pointers, each [head_dim] of the dtype */
+  int weight_orders;         /* 0 (none), 1 (ordinary) or degree + 1 (a series) */
+  void* const* y;            /* forward: degree + 1 pointers, each [batch, heads, length, head_dim] */
+  const void* const* grad;   /* backward: the cotangent series, laid out as y */
+  void* const* dx;           /* backward: degree + 1 pointers, each [batch, length, heads, head_dim] */
+  void* const* dweight;      /* backward: dweight_orders pointers, each [head_dim] of the dtype */
+  int dweight_orders;        /* 0 (none), 1 (order `degree` of the gradient series alone) or degree + 1 */
+} pt_norm_rope_operand;
+
+/*
+ * RMSNorm of every head and the rotation of its first `rotary` elements by position, for one or two
+ * operands in one launch:  y(t) = R(pos) (w(t) (*) x(t) rsqrt(mean(x(t)^2) + eps)).
+ * R turns the pairs (j, j + rotary / 2), or (2 j, 2 j + 1) where interleaved, by the angle whose cosine
+ * and sine are cos[pos][j], sin[pos][j]: tables [table_rows, rotary / 2] of the arithmetic type.
+ * positions: int64 (device), token (b, l) at positions[b position_batch_stride + l]; null: l. A negative
+ * position is padding (zero rows and gradients), one of table_rows or more gives NaN rows.
+ * batch x length x heads is below 2^31 an operand. No counterpart in the reference: there, F.rms_norm
+ * (/root/reference/src/polytensors/_decompositions.py:14-22), slices, products and a transposing copy.
+ */
+int pt_norm_rope_series_fwd(int dtype, int degree, int n_operands, const pt_norm_rope_operand* operands,
+                            int64_t batch, int64_t length, int64_t head_dim, int64_t rotary, int interleaved,
+                            const void* cos, const void* sin, int64_t table_rows, const int64_t* positions,
+                            int64_t position_batch_stride, double eps, void* stream);
+/*
+ * Its gradient series, dx(t) = J(x(t))^T grad(t), and the weights' dw(t) = sum over rows of the
+ * normalized rows times the turned-back cotangent. workspace: with weight gradients, the sum of
+ * pt_norm_rope_series_bwd_workspace_size over the operands that have one (rows: batch x length x heads).
+ */
+int pt_norm_rope_series_bwd(int dtype, int degree, int n_operands, const pt_norm_rope_operand* operands,
+                            int64_t batch, int64_t length, int64_t head_dim, int64_t rotary, int interleaved,
+                            const void* cos, const void* sin, int64_t table_rows, const int64_t* positions,
+                            int64_t position_batch_stride, double eps, void* workspace, void* stream);
+size_t pt_norm_rope_series_bwd_workspace_size(int dtype, int degree, int64_t rows, int64_t head_dim);
+
+/* Largest number of alternatives of pt_token_log_probs_series_*. */
+#define PT_LOG_PROBS_MAX_TOP 32
+
+/*
+ * Per row of a degree-K series of logits z(t) (laid out as pt_cross_entropy_series_fwd's; softcap as
+ * there, 0 for none): the log probability of tokens[row], the entropy of the row's distribution, the
+ * `top` most probable classes (of the largest constant orders, ties by the lower class) and their log
+ * probabilities.
+ * tokens: [rows] int64. A row whose token is ignore_index has zero results, and -1 in top_tokens; a token
+ * that is no class has log probability NaN.
+ * log_probs, entropy, lse (the log-sum-exp series, for the gradient): K + 1 pointers, each [rows] of the
+ * arithmetic type; top_log_probs: K + 1 pointers, each [rows, top]; top_tokens: [rows, top] int64.
+ * workspace: pt_token_log_probs_series_workspace_size bytes (0: none needed).
+ * Log probabilities and entropy follow the reference's log-softmax series
+ *   (/root/reference/src/polytensors/_plain.py:262-273); it has no alternatives.
+ */
+int pt_token_log_probs_series_fwd(int dtype, int degree, const void* const* logits, int64_t rows,
+                                  int64_t classes, int64_t row_stride, const int64_t* tokens,
+                                  int64_t ignore_index, double softcap, int top, void* const* log_probs,
+                                  void* const* entropy, int64_t* top_tokens, void* const* top_log_probs,
+                                  void* const* lse, void* workspace, void* stream);
+size_t pt_token_log_probs_series_workspace_size(int dtype, int degree, int64_t rows, int64_t classes, int top);
+/*
+ * Gradient series dz(t) = J(z(t))^T c(t) of the cotangents of log_probs, entropy and top_log_probs (each
+ * K + 1 pointers laid out as the output, or null for zero). lse, entropy, top_tokens: the forward's.
+ * dz: K + 1 pointers, each [rows, classes] of `dtype`.
+ */
+int pt_token_log_probs_series_bwd(int dtype, int degree, const void* const* logits, int64_t rows,
+                                  int64_t classes, int64_t row_stride, const int64_t* tokens,
+                                  int64_t ignore_index, double softcap, int top, const int64_t* top_tokens,
+                                  const void* const* lse, const void* const* entropy,
+                                  const void* const* cot_log_probs, const void* const* cot_entropy,
+                                  const void* const* cot_top_log_probs, void* const* dz, void* stream);
 
 /*
  * Streaming probes (measurement only; no counterpart in the reference): the

@@ -3,7 +3,7 @@
 Mirrors ``maybe_decompose`` of the reference
 (/root/reference/src/polytensors/_decompositions.py:52-99): rms_norm,
 cross_entropy and scaled_dot_product_attention are intercepted above autograd
-and sent to their fused entry point when ``eligible``; LayerNorm and the
+and sent to their fused entry point when ``eligible``; LayerNorm, dropout and the
 matrix products (torch.matmul, @, mm, bmm, F.linear) are intercepted here too,
 so they reach the Cauchy-product kernel without the copies the
 CompositeImplicit matmul decomposition makes. Where the reference falls back to
@@ -15,12 +15,13 @@ import torch
 import torch.nn.functional as F
 
 from ._tensor import PolyTensor
-from . import _fused_attention, _fused_cross_entropy, _fused_matmul, _fused_norm
+from . import _fused_attention, _fused_cross_entropy, _fused_dropout, _fused_matmul, _fused_norm
 
 _RMS_NORM = frozenset((F.rms_norm, torch.rms_norm))
 _LAYER_NORM = frozenset((F.layer_norm, torch.layer_norm))
 _ATTENTION = frozenset((F.scaled_dot_product_attention,))
 _CROSS_ENTROPY = frozenset((F.cross_entropy,))
+_DROPOUT = frozenset((F.dropout, torch.dropout))
 _CROSS_ENTROPY_ARGS = ("input", "target", "weight", "size_average", "ignore_index", "reduce", "reduction",
                        "label_smoothing")
 _MATMUL = frozenset((torch.matmul, torch.Tensor.matmul, torch.Tensor.__matmul__, torch.Tensor.__rmatmul__,
@@ -83,6 +84,13 @@ def maybe_decompose(function, args, kwargs):
         return _fused_attention.attention_checked(bound["query"], bound["key"], bound["value"],
                                           attn_mask=bound.get("attn_mask"), is_causal=bound.get("is_causal", False),
                                           scale=bound.get("scale"))
+
+    if function in _DROPOUT:
+        names = ("input", "p", "train") if function is torch.dropout else ("input", "p", "training", "inplace")
+        bound = dict(zip(names, args))
+        bound.update(kwargs)
+        return _fused_dropout.functional(bound["input"], bound.get("p", 0.5), bound.get("train", bound.get("training", True)),
+                                         bound.get("inplace", False))
 
     if function in _MATMUL:
         if _needs_grad(args, kwargs):

@@ -15,7 +15,7 @@ import torch
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libpolytaylor.so")
 # the operators' PyTorch registration (csrc/torch_ops.cpp), linked with libpolytaylor.so
 TORCH_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libpolytaylor_torch.so")
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 PT_OK, PT_INVALID_ARGUMENT, PT_UNSUPPORTED, PT_DEVICE_ERROR = 0, 1, 2, 3
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -89,8 +89,27 @@ SIGNATURES = {
     "pt_rms_norm_series_bwd": (_c_int, [_c_int, _c_int, _c_vpp, _c_vpp, _c_vpp, _c_i64, _c_i64, _c_dbl, _c_vp]),
     "pt_norm_series_bwd_weighted": (_c_int, [_c_int, _c_int, _c_int, _c_vpp, _c_vpp, _c_vp, _c_vpp, _c_i64, _c_i64, _c_dbl,
                                              _c_vp]),
+    "pt_dropout_series": (_c_int, [_c_int, _c_int, _c_vpp, _c_vpp, _c_i64, _c_dbl, _c_vp, _c_vp]),
+    "pt_norm_rope_series_fwd": (_c_int, [_c_int, _c_int, _c_int, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_vp,
+                                         _c_vp, _c_i64, _c_vp, _c_i64, _c_dbl, _c_vp]),
+    "pt_norm_rope_series_bwd": (_c_int, [_c_int, _c_int, _c_int, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_vp,
+                                         _c_vp, _c_i64, _c_vp, _c_i64, _c_dbl, _c_vp, _c_vp]),
+    "pt_norm_rope_series_bwd_workspace_size": (ctypes.c_size_t, [_c_int, _c_int, _c_i64, _c_i64]),
+    "pt_token_log_probs_series_fwd": (_c_int, [_c_int, _c_int, _c_vpp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_dbl,
+                                               _c_int, _c_vpp, _c_vpp, _c_vp, _c_vpp, _c_vpp, _c_vp, _c_vp]),
+    "pt_token_log_probs_series_workspace_size": (ctypes.c_size_t, [_c_int, _c_int, _c_i64, _c_i64, _c_int]),
+    "pt_token_log_probs_series_bwd": (_c_int, [_c_int, _c_int, _c_vpp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_dbl,
+                                               _c_int, _c_vp, _c_vpp, _c_vpp, _c_vpp, _c_vpp, _c_vpp, _c_vpp, _c_vp]),
     "pt_layer_norm_series_bwd": (_c_int, [_c_int, _c_int, _c_vpp, _c_vpp, _c_vpp, _c_i64, _c_i64, _c_dbl, _c_vp]),
 }
+
+
+class NormRopeOperand(ctypes.Structure):
+    """pt_norm_rope_operand of include/polytaylor.h."""
+
+    _fields_ = [("x", _c_vpp), ("stride_b", _c_i64), ("stride_l", _c_i64), ("stride_h", _c_i64), ("heads", _c_i64),
+                ("weight", _c_vpp), ("weight_orders", _c_int), ("y", _c_vpp), ("grad", _c_vpp), ("dx", _c_vpp),
+                ("dweight", _c_vpp), ("dweight_orders", _c_int)]
 
 
 class LibraryMissingError(RuntimeError):

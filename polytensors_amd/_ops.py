@@ -44,12 +44,25 @@ SCHEMAS = {
                            "-> (Tensor, Tensor)"),
     "activation_series_backward": "(Tensor[] grad, Tensor[] saved, str kind) -> Tensor",
     "series_binary": "(Tensor[] a, Tensor[] b, str op) -> Tensor",
+    "dropout_series": "(Tensor[] x, Tensor seed, float p) -> Tensor",
+    "norm_rope_series": ("(Tensor[] q, Tensor[] k, Tensor cos, Tensor sin, Tensor? positions, Tensor[] q_weight, "
+                         "Tensor[] k_weight, float eps, bool interleaved) -> (Tensor, Tensor)"),
+    "norm_rope_series_backward": ("(Tensor[] q, Tensor[] k, Tensor[] q_grad, Tensor[] k_grad, Tensor cos, Tensor sin, "
+                                  "Tensor? positions, Tensor[] q_weight, Tensor[] k_weight, float eps, bool interleaved, "
+                                  "int dq_weight, int dk_weight) -> (Tensor, Tensor, Tensor, Tensor)"),
+    "token_log_probs_series": ("(Tensor[] z, Tensor tokens, int ignore_index, float softcap, int top) "
+                               "-> (Tensor, Tensor, Tensor, Tensor, Tensor)"),
+    "token_log_probs_series_backward": ("(Tensor[] z, Tensor tokens, int ignore_index, float softcap, Tensor lse, "
+                                        "Tensor entropy, Tensor? top_tokens, Tensor[] cot_log_probs, "
+                                        "Tensor[] cot_entropy, Tensor[] cot_top) -> Tensor"),
 }
 # The same results as a tensor per order, for calls whose coefficients autograd records: their
 # cotangents arrive order by order as they are. The slices of a stacked result are differentiated by
 # stacking their cotangents, a copy of the whole series for every operation.
-ORDERS = ("norm_series", "cauchy_matmul", "activation_series", "series_binary")
+ORDERS = ("norm_series", "cauchy_matmul", "activation_series", "series_binary", "dropout_series")
 SCHEMAS.update({f"{name}_orders": SCHEMAS[name][:-len("Tensor")] + "Tensor[]" for name in ORDERS})
+# (the queries' orders, then the keys')
+SCHEMAS["norm_rope_series_orders"] = SCHEMAS["norm_rope_series"][:-len("(Tensor, Tensor)")] + "Tensor[]"
 
 _fallback = []   # the Python library object of the stand-in schemas (kept alive)
 
@@ -308,6 +321,64 @@ def _(x, kind):
 @torch.library.register_fake(f"{NAMESPACE}::series_binary_orders")
 def _(a, b, op):
     return [a[0].new_empty(a[0].shape) for _ in a]
+
+
+# ---------------------------------------------------------------------------
+# Dropout, per-head norm and rotation, token log probabilities
+
+dropout_series = _op("dropout_series")
+dropout_series_orders = _op("dropout_series_orders")
+norm_rope_series = _op("norm_rope_series")
+norm_rope_series_orders = _op("norm_rope_series_orders")
+norm_rope_series_backward = _op("norm_rope_series_backward")
+token_log_probs_series = _op("token_log_probs_series")
+token_log_probs_series_backward = _op("token_log_probs_series_backward")
+
+
+@torch.library.register_fake(f"{NAMESPACE}::dropout_series")
+def _(x, seed, p):
+    return x[0].new_empty((len(x), *x[0].shape))
+
+
+@torch.library.register_fake(f"{NAMESPACE}::dropout_series_orders")
+def _(x, seed, p):
+    return [x[0].new_empty(x[0].shape) for _ in x]
+
+
+def _heads_first(x):
+    batch, length, heads, dim = x.shape
+    return batch, heads, length, dim
+
+
+@torch.library.register_fake(f"{NAMESPACE}::norm_rope_series")
+def _(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved):
+    return (q[0].new_empty((len(q), *_heads_first(q[0]))),
+            q[0].new_empty((len(k), *_heads_first(k[0])) if k else (0,)))
+
+
+@torch.library.register_fake(f"{NAMESPACE}::norm_rope_series_orders")
+def _(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved):
+    return [c.new_empty(_heads_first(c)) for c in (*q, *k)]
+
+
+@torch.library.register_fake(f"{NAMESPACE}::norm_rope_series_backward")
+def _(q, k, q_grad, k_grad, cos, sin, positions, q_weight, k_weight, eps, interleaved, dq_weight, dk_weight):
+    dim = q[0].shape[-1]
+    return (q[0].new_empty((len(q), *q[0].shape)), q[0].new_empty((len(k), *k[0].shape) if k else (0,)),
+            q[0].new_empty((dq_weight, dim)), q[0].new_empty((dk_weight, dim) if k else (0,)))
+
+
+@torch.library.register_fake(f"{NAMESPACE}::token_log_probs_series")
+def _(z, tokens, ignore_index, softcap, top):
+    rows, acc = z[0].shape[0], _acc_dtype(z[0].dtype)
+    line = lambda: z[0].new_empty((len(z), rows), dtype=acc)   # noqa: E731
+    return (line(), line(), z[0].new_empty((rows, top), dtype=torch.int64),
+            z[0].new_empty((len(z), rows, top), dtype=acc), line())
+
+
+@torch.library.register_fake(f"{NAMESPACE}::token_log_probs_series_backward")
+def _(z, tokens, ignore_index, softcap, lse, entropy, top_tokens, cot_log_probs, cot_entropy, cot_top):
+    return z[0].new_empty((len(z), *z[0].shape))
 
 
 # ---------------------------------------------------------------------------
@@ -704,6 +775,106 @@ def _binary_backward(ctx, grad):
 
 torch.library.register_autograd(f"{NAMESPACE}::series_binary", _binary_backward, setup_context=_binary_setup)
 torch.library.register_autograd(f"{NAMESPACE}::series_binary_orders", _binary_backward, setup_context=_binary_setup)
+
+
+def _dropout_setup(ctx, inputs, output):
+    x, seed, p = inputs
+    ctx.save_for_backward(seed)
+    ctx.meta = (len(x), p)
+
+
+def _dropout_backward(ctx, grad):
+    # the mask acts on each order alone: the cotangents' dropout, order by order (differentiable again)
+    (seed,) = ctx.saved_tensors
+    n, p = ctx.meta
+    cots = _reversed(grad)[::-1]
+    return _returned(ctx, list(dropout_series_orders(cots, seed, p)))
+
+
+torch.library.register_autograd(f"{NAMESPACE}::dropout_series", _dropout_backward, setup_context=_dropout_setup)
+torch.library.register_autograd(f"{NAMESPACE}::dropout_series_orders", _dropout_backward, setup_context=_dropout_setup)
+
+
+def _norm_rope_setup(ctx, inputs, output):
+    q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved = inputs
+    ctx.save_for_backward(*q, *k, *q_weight, *k_weight, cos, sin, *([] if positions is None else [positions]))
+    ctx.meta = (len(q), len(k), len(q_weight), len(k_weight), eps, interleaved, _grads_flag(q_weight), _grads_flag(k_weight))
+
+
+def _norm_rope_backward(ctx, *grads):
+    _once("qk_norm_rope")
+    nq, nk, nqw, nkw, eps, interleaved, need_qw, need_kw = ctx.meta
+    saved = list(ctx.saved_tensors)
+    take = lambda n: [saved.pop(0) for _ in range(n)]   # noqa: E731
+    q, k, qw, kw = take(nq), take(nk), take(nqw), take(nkw)
+    cos, sin = take(2)
+    positions = saved[0] if saved else None
+    if len(grads) == 1:   # the tensor-per-order form
+        gq, gk = list(grads[0][:nq]), list(grads[0][nq:])
+    else:
+        gq, gk = (None if g is None else list(g.unbind(0)) for g in grads)
+    results = norm_rope_gradients([(q, gq, qw, need_qw), (k, gk, kw, need_kw)], cos, sin, positions, eps, interleaved,
+                                  reverse=True)
+    dx, dw = [], []
+    for (x, w, got) in ((q, qw, results[0]), (k, kw, results[1])):
+        dx.append([None] * len(x) if got is None or got[0] is None else _read_back(got[0], len(x)))
+        if got is None or got[1] is None:
+            dw.append([None] * len(w))
+        else:   # an ordinary weight's is the last order of the gradient series
+            dw.append([got[1][0]] if len(w) == 1 else _read_back(got[1], len(w)))
+    return _returned(ctx, dx[0], dx[1], None, None, None, dw[0], dw[1])
+
+
+def norm_rope_gradients(operands, cos, sin, positions, eps, interleaved, reverse):
+    """(dx, dw) gradient series of each operand (coefficients, cotangents, weight coefficients, whether the
+    weight's gradient is wanted): None for an operand without orders or cotangents. ``reverse``: the
+    cotangents are those of coefficient autograd, which the kernel takes in reverse order; an ordinary
+    weight's gradient is then one order, otherwise (a gradient series) a weight's has all."""
+    calls, slots = [], []
+    for i, (x, g, w, need) in enumerate(operands):
+        if not x or g is None or all(c is None for c in g):
+            continue
+        cots = _reversed(g)
+        want = 0 if not (need and w) else (1 if reverse and len(w) == 1 else len(x))
+        calls.append((x, cots if reverse else cots[::-1], w, want))
+        slots.append(i)
+    results = [None] * len(operands)
+    if not calls:
+        return results
+    (x, g, w, want) = calls[0]
+    (x2, g2, w2, want2) = calls[1] if len(calls) > 1 else ([], [], [], 0)
+    out = norm_rope_series_backward(x, x2, g, g2, cos, sin, positions, w, w2, eps, interleaved, want, want2)
+    for j, i in enumerate(slots):
+        results[i] = (out[j], out[2 + j] if calls[j][3] else None)
+    return results
+
+
+torch.library.register_autograd(f"{NAMESPACE}::norm_rope_series", _norm_rope_backward, setup_context=_norm_rope_setup)
+torch.library.register_autograd(f"{NAMESPACE}::norm_rope_series_orders", _norm_rope_backward,
+                                setup_context=_norm_rope_setup)
+
+
+def _log_probs_setup(ctx, inputs, output):
+    z, tokens, ignore_index, softcap, top = inputs
+    log_probs, entropy, top_tokens, top_log_probs, lse = output
+    ctx.mark_non_differentiable(top_tokens, lse)
+    ctx.save_for_backward(*z, tokens, entropy, top_tokens, lse)
+    ctx.meta = (len(z), ignore_index, softcap, top)
+
+
+def _log_probs_backward(ctx, grad_log_probs, grad_entropy, grad_tokens, grad_top, grad_lse):
+    _once("token_log_probs")
+    n, ignore_index, softcap, top = ctx.meta
+    saved = ctx.saved_tensors
+    z, (tokens, entropy, top_tokens, lse) = list(saved[:n]), saved[n:]
+    cots = [[] if g is None or (i == 2 and top == 0) else [c.contiguous() for c in g.to(lse.dtype).flip(0).unbind(0)]
+            for i, g in enumerate((grad_log_probs, grad_entropy, grad_top))]
+    dz = token_log_probs_series_backward(z, tokens, ignore_index, softcap, lse, entropy, top_tokens, *cots)
+    return _returned(ctx, _read_back(dz, n))
+
+
+torch.library.register_autograd(f"{NAMESPACE}::token_log_probs_series", _log_probs_backward,
+                                setup_context=_log_probs_setup)
 
 
 # The complex-direction plumbing is linear in its inputs. Its gradients follow torch's

@@ -288,6 +288,51 @@ class PolyTensor(torch.Tensor):
 
         return cross_entropy(logits, target, softcap=softcap, ignore_index=ignore_index, reduction=reduction)
 
+    @staticmethod
+    def qk_norm_rope(query, key, cos, sin, positions=None, query_weight=None, key_weight=None, eps=None,
+                     interleaved=False):
+        """Queries and keys ready for attention: RMSNorm of every head and rotation by position in one pass.
+
+        ``query`` (B, L, H, D) and ``key`` (B, L, G, D), for instance the parts of a projection's output,
+        become (B, H, L, D) and (B, G, L, D):  R(position) (weight * x * rsqrt(mean(x^2) + eps)) over
+        each head. ``cos``, ``sin`` (P, rotary / 2), float32 (float64 for float64 operands): R turns the
+        first ``rotary`` elements of a head, the pairs (j, j + rotary / 2), or (2 j, 2 j + 1) with
+        ``interleaved``, by the angles of the token's position. ``positions``: int64 (L,) or (B, L),
+        0..L-1 by default; a negative one is padding (zero rows, no gradient), one of P or more gives NaN.
+        ``eps`` defaults to ``torch.finfo(dtype).eps``. Heads have at most 256 elements; an operand and a
+        weight may be a PolyTensor or an ordinary tensor; degrees up to 8.
+        """
+        from ._fused_norm_rope import qk_norm_rope
+
+        return qk_norm_rope(query, key, cos, sin, positions, query_weight, key_weight, eps, interleaved)
+
+    @staticmethod
+    def token_log_probs(logits, tokens, top=0, softcap=None, ignore_index=-100):
+        """Log probabilities of given tokens, entropies and most probable alternatives of (..., C) logits.
+
+        Returns ``TokenLogProbs(log_probs, entropy, top_tokens, top_log_probs)``: series of the tokens' shape
+        (...), and with ``top`` (at most 32) the classes (..., top) of the largest logits' constant orders
+        in order, ties by the lower class, with their log-probability series (None without). At least
+        float32. ``softcap`` caps the logits as in ``cross_entropy``. A token equal to ``ignore_index`` has
+        zero results, -1 as alternatives and no gradient; one that is no class has log probability NaN. Degrees up to 8.
+        """
+        from ._fused_log_probs import token_log_probs
+
+        return token_log_probs(logits, tokens, top=top, softcap=softcap, ignore_index=ignore_index)
+
+    @staticmethod
+    def dropout(input, p=0.5, seed=None):
+        """Each element zero with probability ``p``, else times 1 / (1 - p): the same elements in every order.
+
+        The mask is a function of ``seed`` and the element's row-major index (Philox4x32-10), so it is not
+        stored and the same seed gives the same mask: an int, or an int64 tensor of one element on the
+        input's device (which a captured graph reads at every replay); by default drawn from torch's
+        generator. Degrees up to 16. ``torch.nn.functional.dropout`` in training comes here too.
+        """
+        from ._fused_dropout import dropout
+
+        return dropout(input, p, seed)
+
     def backward(self, gradient=None, retain_graph=None, create_graph=False, inputs=None):
         """Reverse mode through the series (/root/reference/src/polytensors/_tensor.py:325-338).
 

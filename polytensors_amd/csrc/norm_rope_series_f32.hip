@@ -1,0 +1,7 @@
+// Instantiates the per-head norm and rotation kernels for one storage type.
+#include "norm_rope_series.inl"
+
+namespace pt {
+template int launch_norm_rope<float>(const NormRopeArgs&);
+template int launch_norm_rope_bwd<float>(const NormRopeArgs&);
+}  // namespace pt

@@ -1,0 +1,7 @@
+// Instantiates the token log-probability kernels for one storage type.
+#include "token_log_probs_series.inl"
+
+namespace pt {
+template int launch_log_probs<_Float16>(const LogProbArgs&);
+template int launch_log_probs_bwd<_Float16>(const LogProbBwdArgs&);
+}  // namespace pt

@@ -1,0 +1,7 @@
+// Instantiates the token log-probability kernels for one storage type.
+#include "token_log_probs_series.inl"
+
+namespace pt {
+template int launch_log_probs<double>(const LogProbArgs&);
+template int launch_log_probs_bwd<double>(const LogProbBwdArgs&);
+}  // namespace pt

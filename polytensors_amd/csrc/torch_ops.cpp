@@ -801,6 +801,282 @@ TensorList series_binary_orders(const TensorList& a, const TensorList& b, c10::s
   return series_binary_out(true, a, b, op).orders;
 }
 
+// ---- Dropout -------------------------------------------------------------------
+
+SeriesOut dropout_series_out(bool separate, const TensorList& x, const Tensor& seed, double p) {
+  check_abi();
+  check_series("dropout_series", x);
+  TORCH_CHECK_VALUE(seed.scalar_type() == at::kLong && seed.numel() == 1 && seed.device() == x[0].device(),
+                    "dropout_series: seed must be one int64 on the operand's device");
+  TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "dropout_series: p must be in [0, 1]");
+  const int64_t orders = static_cast<int64_t>(x.size());
+  c10::DeviceGuard guard(x[0].device());
+  SeriesOut out = series_out(separate, orders, x[0].sizes(), x[0].options());
+  check_status(pt_dropout_series(dtype_code(x[0].scalar_type()), static_cast<int>(orders), cptrs(x).data(),
+                                 out.ptrs.data(), x[0].numel(), p, seed.data_ptr<int64_t>(), stream_of(x[0])),
+               "dropout_series");
+  return out;
+}
+
+Tensor dropout_series(const TensorList& x, const Tensor& seed, double p) {
+  return dropout_series_out(false, x, seed, p).stacked;
+}
+
+TensorList dropout_series_orders(const TensorList& x, const Tensor& seed, double p) {
+  return dropout_series_out(true, x, seed, p).orders;
+}
+
+// ---- Per-head norm and rotation --------------------------------------------------
+
+// An operand [batch, length, heads, D]: any strides common to its orders, a head's elements side by side.
+void check_heads(const std::string& name, const TensorList& x, const Tensor& first) {
+  for (const Tensor& t : x) {
+    TORCH_CHECK_VALUE(t.dim() == 4 && has_code(t.scalar_type()), name, ": coefficients must be floating [batch, length, heads, D]");
+    TORCH_CHECK_VALUE(t.scalar_type() == first.scalar_type() && t.device() == first.device(), name,
+                      ": coefficients must share dtype and device");
+    TORCH_CHECK_VALUE(t.sizes() == x[0].sizes() && t.strides() == x[0].strides() && (t.size(3) <= 1 || t.stride(3) == 1), name,
+                      ": coefficients must share shape and strides, with unit stride in a head");
+  }
+  TORCH_CHECK_VALUE(x[0].size(0) == first.size(0) && x[0].size(1) == first.size(1) && x[0].size(3) == first.size(3), name,
+                    ": operands must share batch, length and head size");
+}
+
+struct RopeInputs {
+  std::vector<const void*> x, w, g;
+  std::vector<void*> y, dw;
+};
+
+struct RopeCall {
+  std::vector<RopeInputs> in;
+  std::vector<pt_norm_rope_operand> ops;
+  int64_t batch, length, dim, rotary, position_stride;
+  const int64_t* positions;
+};
+
+RopeCall rope_call(const std::string& name, const TensorList& q, const TensorList& k, const Tensor& cos, const Tensor& sin,
+                   const c10::optional<Tensor>& positions, const TensorList& q_weight, const TensorList& k_weight) {
+  TORCH_CHECK_VALUE(!q.empty() && (k.empty() || k.size() == q.size()), name, ": operands need the same number of orders");
+  const Tensor& first = q[0];
+  RopeCall c{};
+  for (const TensorList* x : {&q, &k})
+    if (!x->empty()) check_heads(name, *x, first);
+  c.batch = first.size(0);
+  c.length = first.size(1);
+  c.dim = first.size(3);
+  const at::ScalarType acc = acc_type(first.scalar_type());
+  for (const Tensor* t : {&cos, &sin})
+    TORCH_CHECK_VALUE(t->dim() == 2 && t->scalar_type() == acc && t->device() == first.device() && t->is_contiguous() &&
+                          t->sizes() == cos.sizes(),
+                      name, ": cos and sin must be contiguous [positions, rotary / 2] of the arithmetic type");
+  c.rotary = 2 * cos.size(1);
+  TORCH_CHECK_VALUE(c.rotary <= c.dim, name, ": the tables turn more elements than a head has");
+  if (positions) {
+    const Tensor& p = *positions;
+    TORCH_CHECK_VALUE(p.scalar_type() == at::kLong && p.device() == first.device() && p.is_contiguous() &&
+                          ((p.dim() == 1 && p.size(0) == c.length) ||
+                           (p.dim() == 2 && p.size(0) == c.batch && p.size(1) == c.length)),
+                      name, ": positions must be contiguous int64 [length] or [batch, length]");
+    c.positions = p.data_ptr<int64_t>();
+    c.position_stride = p.dim() == 2 ? c.length : 0;
+  }
+  c.in.resize(k.empty() ? 1 : 2);
+  for (size_t o = 0; o < c.in.size(); ++o) {
+    const TensorList &x = o == 0 ? q : k, &w = o == 0 ? q_weight : k_weight;
+    TORCH_CHECK_VALUE(w.empty() || w.size() == 1 || w.size() == x.size(), name, ": a weight needs 0, 1 or degree+1 coefficients");
+    for (const Tensor& t : w)
+      TORCH_CHECK_VALUE(t.scalar_type() == first.scalar_type() && t.device() == first.device() && t.dim() == 1 &&
+                            t.size(0) == c.dim && t.is_contiguous(),
+                        name, ": weights must be contiguous [D] of the operands' dtype");
+    c.in[o].x = cptrs(x);
+    c.in[o].w = cptrs(w);
+    pt_norm_rope_operand op{};
+    op.x = c.in[o].x.data();
+    op.stride_b = x[0].stride(0);
+    op.stride_l = x[0].stride(1);
+    op.stride_h = x[0].stride(2);
+    op.heads = x[0].size(2);
+    op.weight = w.empty() ? nullptr : c.in[o].w.data();
+    op.weight_orders = static_cast<int>(w.size());
+    c.ops.push_back(op);
+  }
+  return c;
+}
+
+struct RopeOut {
+  SeriesOut q, k;
+};
+
+RopeOut norm_rope_series_out(bool separate, const TensorList& q, const TensorList& k, const Tensor& cos, const Tensor& sin,
+                             const c10::optional<Tensor>& positions, const TensorList& q_weight, const TensorList& k_weight,
+                             double eps, bool interleaved) {
+  check_abi();
+  RopeCall c = rope_call("norm_rope_series", q, k, cos, sin, positions, q_weight, k_weight);
+  const int64_t orders = static_cast<int64_t>(q.size());
+  c10::DeviceGuard guard(q[0].device());
+  RopeOut out;
+  for (size_t o = 0; o < c.ops.size(); ++o) {
+    SeriesOut& y = o == 0 ? out.q : out.k;
+    y = series_out(separate, orders, {c.batch, c.ops[o].heads, c.length, c.dim}, q[0].options());
+    c.ops[o].y = y.ptrs.data();
+  }
+  if (k.empty() && !separate) out.k.stacked = at::empty({0}, q[0].options());
+  if (c.batch * c.length == 0) return out;
+  check_status(pt_norm_rope_series_fwd(dtype_code(q[0].scalar_type()), static_cast<int>(orders) - 1,
+                                       static_cast<int>(c.ops.size()), c.ops.data(), c.batch, c.length, c.dim, c.rotary,
+                                       interleaved ? 1 : 0, cos.data_ptr(), sin.data_ptr(), cos.size(0), c.positions,
+                                       c.position_stride, eps, stream_of(q[0])),
+               "norm_rope_series");
+  return out;
+}
+
+std::tuple<Tensor, Tensor> norm_rope_series(const TensorList& q, const TensorList& k, const Tensor& cos, const Tensor& sin,
+                                            const c10::optional<Tensor>& positions, const TensorList& q_weight,
+                                            const TensorList& k_weight, double eps, bool interleaved) {
+  RopeOut out = norm_rope_series_out(false, q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved);
+  return {out.q.stacked, out.k.stacked};
+}
+
+// The orders of the queries, then those of the keys.
+TensorList norm_rope_series_orders(const TensorList& q, const TensorList& k, const Tensor& cos, const Tensor& sin,
+                                   const c10::optional<Tensor>& positions, const TensorList& q_weight,
+                                   const TensorList& k_weight, double eps, bool interleaved) {
+  RopeOut out = norm_rope_series_out(true, q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved);
+  out.q.orders.insert(out.q.orders.end(), out.k.orders.begin(), out.k.orders.end());
+  return out.q.orders;
+}
+
+// dq, dk and the weights' gradients (dq_weight, dk_weight: 0, 1 or every order).
+std::tuple<Tensor, Tensor, Tensor, Tensor> norm_rope_series_backward(
+    const TensorList& q, const TensorList& k, const TensorList& q_grad, const TensorList& k_grad, const Tensor& cos,
+    const Tensor& sin, const c10::optional<Tensor>& positions, const TensorList& q_weight, const TensorList& k_weight,
+    double eps, bool interleaved, int64_t dq_weight, int64_t dk_weight) {
+  check_abi();
+  const std::string name = "norm_rope_series_backward";
+  RopeCall c = rope_call(name, q, k, cos, sin, positions, q_weight, k_weight);
+  const int64_t orders = static_cast<int64_t>(q.size());
+  c10::DeviceGuard guard(q[0].device());
+  Tensor dx[2], dw[2];
+  size_t wbytes = 0;
+  const int code = dtype_code(q[0].scalar_type());
+  dx[1] = at::empty({0}, q[0].options());
+  dw[1] = at::empty({0}, q[0].options());
+  for (size_t o = 0; o < c.ops.size(); ++o) {
+    const TensorList& g = o == 0 ? q_grad : k_grad;
+    pt_norm_rope_operand& op = c.ops[o];
+    check_series(name + " grad", g, q[0].scalar_type());
+    TORCH_CHECK_VALUE(static_cast<int64_t>(g.size()) == orders && g[0].device() == q[0].device() &&
+                          g[0].sizes() == at::IntArrayRef({c.batch, op.heads, c.length, c.dim}),
+                      name, ": cotangents must be [batch, heads, length, D], an order each");
+    const int64_t want = o == 0 ? dq_weight : dk_weight;
+    TORCH_CHECK_VALUE(want == 0 || want == 1 || want == orders, name, ": weight gradients need 0, 1 or degree+1 orders");
+    dx[o] = at::empty({orders, c.batch, c.length, op.heads, c.dim}, q[0].options());
+    dw[o] = c.batch * c.length == 0 ? at::zeros({want, c.dim}, q[0].options()) : at::empty({want, c.dim}, q[0].options());
+    c.in[o].g = cptrs(g);
+    c.in[o].y = slices(dx[o]);
+    c.in[o].dw = slices(dw[o]);
+    op.grad = c.in[o].g.data();
+    op.dx = c.in[o].y.data();
+    op.dweight = c.in[o].dw.data();
+    op.dweight_orders = static_cast<int>(want);
+    if (want > 0)
+      wbytes += pt_norm_rope_series_bwd_workspace_size(code, static_cast<int>(orders) - 1, c.batch * c.length * op.heads, c.dim);
+  }
+  if (c.batch * c.length == 0) return {dx[0], dx[1], dw[0], dw[1]};
+  Tensor workspace = at::empty({static_cast<int64_t>(std::max<size_t>(1, wbytes))}, q[0].options().dtype(at::kByte));
+  check_status(pt_norm_rope_series_bwd(code, static_cast<int>(orders) - 1, static_cast<int>(c.ops.size()), c.ops.data(),
+                                       c.batch, c.length, c.dim, c.rotary, interleaved ? 1 : 0, cos.data_ptr(),
+                                       sin.data_ptr(), cos.size(0), c.positions, c.position_stride, eps,
+                                       workspace.data_ptr(), stream_of(q[0])),
+               name);
+  return {dx[0], dx[1], dw[0], dw[1]};
+}
+
+// ---- Token log probabilities -------------------------------------------------------
+
+void check_tokens(const std::string& name, const Tensor& tokens, const Tensor& first) {
+  TORCH_CHECK_VALUE(tokens.scalar_type() == at::kLong && tokens.dim() == 1 && tokens.size(0) == first.size(0) &&
+                        tokens.is_contiguous() && tokens.device() == first.device(),
+                    name, ": tokens must be contiguous int64 [N] on the logits' device");
+}
+
+// Log probabilities and entropy [K+1, N], the alternatives [N, top] and their log probabilities
+// [K+1, N, top], and the log-sum-exp series [K+1, N].
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_log_probs_series(const TensorList& z, const Tensor& tokens,
+                                                                          int64_t ignore_index, double softcap,
+                                                                          int64_t top) {
+  check_abi();
+  const std::string name = "token_log_probs_series";
+  check_logit_rows(name, z);
+  const Tensor& first = z[0];
+  check_tokens(name, tokens, first);
+  TORCH_CHECK_VALUE(top >= 0 && top <= PT_LOG_PROBS_MAX_TOP && top <= first.size(1), name,
+                    ": top must be in 0..", PT_LOG_PROBS_MAX_TOP, " and at most the number of classes");
+  const int64_t orders = static_cast<int64_t>(z.size()), rows = first.size(0), classes = first.size(1);
+  c10::DeviceGuard guard(first.device());
+  const auto acc = first.options().dtype(acc_type(first.scalar_type()));
+  Tensor log_probs = at::empty({orders, rows}, acc), entropy = at::empty({orders, rows}, acc),
+         lse = at::empty({orders, rows}, acc);
+  Tensor top_tokens = at::empty({rows, top}, first.options().dtype(at::kLong));
+  Tensor top_log_probs = at::empty({orders, rows, top}, acc);
+  const int code = dtype_code(first.scalar_type());
+  const size_t wbytes = pt_token_log_probs_series_workspace_size(code, static_cast<int>(orders) - 1, rows, classes,
+                                                                 static_cast<int>(top));
+  Tensor workspace;
+  if (wbytes > 0) workspace = at::empty({static_cast<int64_t>(wbytes)}, first.options().dtype(at::kByte));
+  check_status(pt_token_log_probs_series_fwd(
+                   code, static_cast<int>(orders) - 1, cptrs(z).data(), rows, classes, rows ? first.stride(0) : classes,
+                   tokens.data_ptr<int64_t>(), ignore_index, softcap, static_cast<int>(top), slices(log_probs).data(),
+                   slices(entropy).data(), top_tokens.data_ptr<int64_t>(), slices(top_log_probs).data(),
+                   slices(lse).data(), wbytes > 0 ? workspace.data_ptr() : nullptr, stream_of(first)),
+               name);
+  return {log_probs, entropy, top_tokens, top_log_probs, lse};
+}
+
+Tensor token_log_probs_series_backward(const TensorList& z, const Tensor& tokens, int64_t ignore_index, double softcap,
+                                       const Tensor& lse, const Tensor& entropy, const c10::optional<Tensor>& top_tokens,
+                                       const TensorList& cot_log_probs, const TensorList& cot_entropy,
+                                       const TensorList& cot_top) {
+  check_abi();
+  const std::string name = "token_log_probs_series_backward";
+  check_logit_rows(name, z);
+  const Tensor& first = z[0];
+  check_tokens(name, tokens, first);
+  const int64_t orders = static_cast<int64_t>(z.size()), rows = first.size(0), classes = first.size(1);
+  const at::ScalarType acc = acc_type(first.scalar_type());
+  auto check_rows = [&](const Tensor& t, const char* what) {
+    TORCH_CHECK_VALUE(t.scalar_type() == acc && t.device() == first.device() && t.is_contiguous() && t.dim() == 2 &&
+                          t.size(0) == orders && t.size(1) == rows,
+                      name, ": ", what, " must be contiguous [K+1, N] of the arithmetic type");
+  };
+  check_rows(lse, "lse");
+  check_rows(entropy, "entropy");
+  const int64_t top = cot_top.empty() ? 0 : cot_top[0].dim() == 2 ? cot_top[0].size(1) : -1;
+  for (const TensorList* cot : {&cot_log_probs, &cot_entropy, &cot_top})
+    for (const Tensor& c : *cot)
+      TORCH_CHECK_VALUE(static_cast<int64_t>(cot->size()) == orders && c.scalar_type() == acc && c.device() == first.device() &&
+                            c.is_contiguous() && c.dim() == (cot == &cot_top ? 2 : 1) && c.size(0) == rows &&
+                            (cot != &cot_top || c.size(1) == top),
+                        name, ": cotangents must be contiguous [N] (or [N, top]) of the arithmetic type, an order each");
+  TORCH_CHECK_VALUE(cot_top.empty() || (top >= 0 && top_tokens && top_tokens->scalar_type() == at::kLong &&
+                                        top_tokens->device() == first.device() && top_tokens->is_contiguous() &&
+                                        top_tokens->sizes() == at::IntArrayRef({rows, top})),
+                    name, ": top_tokens must be contiguous int64 [N, top]");
+  c10::DeviceGuard guard(first.device());
+  Tensor out = at::empty({orders, rows, classes}, first.options());
+  auto ls = slices(lse), es = slices(entropy);
+  std::vector<const void*> lc(ls.begin(), ls.end()), ec(es.begin(), es.end());
+  auto clp = cptrs(cot_log_probs), cent = cptrs(cot_entropy), ctop = cptrs(cot_top);
+  const bool tops = top > 0;
+  check_status(pt_token_log_probs_series_bwd(
+                   dtype_code(first.scalar_type()), static_cast<int>(orders) - 1, cptrs(z).data(), rows, classes,
+                   rows ? first.stride(0) : classes, tokens.data_ptr<int64_t>(), ignore_index, softcap,
+                   static_cast<int>(top), tops ? top_tokens->data_ptr<int64_t>() : nullptr, lc.data(), ec.data(),
+                   cot_log_probs.empty() ? nullptr : clp.data(), cot_entropy.empty() ? nullptr : cent.data(),
+                   tops ? ctop.data() : nullptr, slices(out).data(), stream_of(first)),
+               name);
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(polytensors_amd, m) {
@@ -824,10 +1100,23 @@ TORCH_LIBRARY(polytensors_amd, m) {
         "-> (Tensor, Tensor)");
   m.def("activation_series_backward(Tensor[] grad, Tensor[] saved, str kind) -> Tensor");
   m.def("series_binary(Tensor[] a, Tensor[] b, str op) -> Tensor");
+  m.def("dropout_series(Tensor[] x, Tensor seed, float p) -> Tensor");
+  m.def("norm_rope_series(Tensor[] q, Tensor[] k, Tensor cos, Tensor sin, Tensor? positions, Tensor[] q_weight, "
+        "Tensor[] k_weight, float eps, bool interleaved) -> (Tensor, Tensor)");
+  m.def("norm_rope_series_backward(Tensor[] q, Tensor[] k, Tensor[] q_grad, Tensor[] k_grad, Tensor cos, Tensor sin, "
+        "Tensor? positions, Tensor[] q_weight, Tensor[] k_weight, float eps, bool interleaved, int dq_weight, "
+        "int dk_weight) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("token_log_probs_series(Tensor[] z, Tensor tokens, int ignore_index, float softcap, int top) "
+        "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("token_log_probs_series_backward(Tensor[] z, Tensor tokens, int ignore_index, float softcap, Tensor lse, "
+        "Tensor entropy, Tensor? top_tokens, Tensor[] cot_log_probs, Tensor[] cot_entropy, Tensor[] cot_top) -> Tensor");
   m.def("norm_series_orders(Tensor[] x, Tensor[] weight, Tensor[] bias, int n, float eps, bool layer) -> Tensor[]");
   m.def("cauchy_matmul_orders(Tensor[] a, Tensor[] b, int degree, bool trans_b, Tensor? bias=None) -> Tensor[]");
   m.def("activation_series_orders(Tensor[] x, str kind) -> Tensor[]");
   m.def("series_binary_orders(Tensor[] a, Tensor[] b, str op) -> Tensor[]");
+  m.def("dropout_series_orders(Tensor[] x, Tensor seed, float p) -> Tensor[]");
+  m.def("norm_rope_series_orders(Tensor[] q, Tensor[] k, Tensor cos, Tensor sin, Tensor? positions, Tensor[] q_weight, "
+        "Tensor[] k_weight, float eps, bool interleaved) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(polytensors_amd, CUDA, m) {
@@ -850,4 +1139,11 @@ TORCH_LIBRARY_IMPL(polytensors_amd, CUDA, m) {
   m.impl("cauchy_matmul_orders", &cauchy_matmul_orders);
   m.impl("activation_series_orders", &activation_series_orders);
   m.impl("series_binary_orders", &series_binary_orders);
+  m.impl("dropout_series", &dropout_series);
+  m.impl("dropout_series_orders", &dropout_series_orders);
+  m.impl("norm_rope_series", &norm_rope_series);
+  m.impl("norm_rope_series_orders", &norm_rope_series_orders);
+  m.impl("norm_rope_series_backward", &norm_rope_series_backward);
+  m.impl("token_log_probs_series", &token_log_probs_series);
+  m.impl("token_log_probs_series_backward", &token_log_probs_series_backward);
 }
