@@ -20,50 +20,52 @@ _DTYPES = (torch.float16, torch.bfloat16, torch.float32, torch.float64)
 
 
 def why_ineligible(query, key, cos, sin, positions, query_weight, key_weight, eps):
-    tensors = [x for x in (query, key, query_weight, key_weight) if x is not None]
-    if not all(isinstance(x, torch.Tensor) for x in (*tensors, cos, sin)) or query is None or key is None:
+    operands = [x for x in (query, key, query_weight, key_weight) if x is not None]
+    if query is None or key is None or not all(isinstance(x, torch.Tensor) for x in (*operands, cos, sin)):
         return "query, key, cos, sin and the weights must be tensors"
-    grads = _gate.wrapper_grad(*tensors)
-    reason = _gate.common_reason(tensors, allow_plain_grad=grads, complex_ok=True)
+    reason = _gate.common_reason(operands, allow_plain_grad=_gate.wrapper_grad(*operands), complex_ok=True)
     if reason is not None:
         return reason
-    ordinary = [x for x in (query, key, query_weight, key_weight, cos, sin)
-                if x is not None and not isinstance(x, PolyTensor)]
-    if _gate.wrapper_grad(*ordinary):
-        return ("an ordinary (non-PolyTensor) operand or weight requires grad: its gradient would be a series, which "
-                "autograd cannot hand to it (make it a PolyTensor, or use coefficient_autograd)")
-    if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
-        return "no gradient flows to the cos and sin tables"
-    if any(_gate.transformed(x) for x in ordinary):
-        return "function transforms are not supported"
-    dtype = _gate.real_dtype(query.dtype)
+    dtype, device = _gate.real_dtype(query.dtype), query.device
     if dtype not in _DTYPES:
         return f"dtype {query.dtype} is not supported (float32, float64, bfloat16 or float16)"
-    for x in tensors:
-        if any(_gate.real_dtype(c.dtype) != dtype for c in _gate.coefficients(x, 0)):
+    acc = torch.float64 if dtype == torch.float64 else torch.float32
+    grads = torch.is_grad_enabled()
+    for x in operands:   # (a series' higher orders share one dtype: its last order stands for them)
+        series = isinstance(x, PolyTensor)
+        if x.dtype != dtype or (series and _gate.real_dtype(x.coeffs[-1].dtype) != dtype):
             return "query, key and the weights must share one dtype"
-        if x.device != query.device:
+        if x.device != device:
             return "operands and weights must be on one device"
-    if query.ndim != 4 or key.ndim != 4 or query.shape[:2] != key.shape[:2] or query.shape[3] != key.shape[3]:
+        if not series:
+            if grads and _gate.wrapper_grad(x):
+                return ("an ordinary (non-PolyTensor) operand or weight requires grad: its gradient would be a series, which "
+                        "autograd cannot hand to it (make it a PolyTensor, or use coefficient_autograd)")
+            if _gate.transformed(x):
+                return "function transforms are not supported"
+    shape, key_shape = query.shape, key.shape
+    if len(shape) != 4 or len(key_shape) != 4 or shape[:2] != key_shape[:2] or shape[3] != key_shape[3]:
         return "query and key must be (B, L, H, D) and (B, L, G, D)"
-    dim = query.shape[3]
-    if not 1 <= dim <= MAX_HEAD or query.shape[2] == 0 or key.shape[2] == 0:
+    batch, length, heads, dim = shape
+    if not 1 <= dim <= MAX_HEAD or heads == 0 or key_shape[2] == 0:
         return f"heads of 1..{MAX_HEAD} elements, at least one head each"
-    if max(query.shape[2], key.shape[2]) * query.shape[0] * query.shape[1] >= 2 ** 31:
+    if max(heads, key_shape[2]) * batch * length >= 2 ** 31:
         return "more than 2^31 - 1 heads"
     for w in (query_weight, key_weight):
         if w is not None and tuple(w.shape) != (dim,):
             return "weights must be (D,)"
-    acc = torch.float64 if dtype == torch.float64 else torch.float32
     for t in (cos, sin):
-        if isinstance(t, PolyTensor) or t.dtype != acc or t.device != query.device or t.ndim != 2 or t.shape != cos.shape \
+        if isinstance(t, PolyTensor) or t.dtype != acc or t.device != device or t.ndim != 2 or t.shape != cos.shape \
                 or 2 * t.shape[1] > dim:
             return f"cos and sin must be ordinary {acc} (P, rotary / 2) on the operands' device, rotary at most D"
-    if positions is not None:
-        if isinstance(positions, PolyTensor) or not isinstance(positions, torch.Tensor) or positions.dtype != torch.int64 or \
-                positions.device != query.device or \
-                tuple(positions.shape) not in ((query.shape[1],), (1, query.shape[1]), tuple(query.shape[:2])):
-            return "positions must be an ordinary int64 (L,) or (B, L) on the operands' device"
+        if _gate.transformed(t):
+            return "function transforms are not supported"
+        if grads and t.requires_grad:
+            return "no gradient flows to the cos and sin tables"
+    if positions is not None and (
+            isinstance(positions, PolyTensor) or not isinstance(positions, torch.Tensor) or positions.dtype != torch.int64 or
+            positions.device != device or tuple(positions.shape) not in ((length,), (1, length), (batch, length))):
+        return "positions must be an ordinary int64 (L,) or (B, L) on the operands' device"
     if isinstance(eps, bool) or not isinstance(eps, (int, float)) or not 0.0 <= eps < float("inf"):
         return "eps must be a finite number of at least 0"
     return None
@@ -110,7 +112,7 @@ class _SeriesNormRope(torch.autograd.Function):
             cots = list(g.coeffs) if isinstance(g, PolyTensor) else [g]
             cots = [c.to(x.dtype) for c in cots] + [None] * (x.degree + 1 - len(cots))
             operands.append((_heads(x.coeffs), cots, _weight(w), need))
-        results = _ops.norm_rope_gradients(operands, cos, sin, positions, eps, interleaved, reverse=False)
+        results = _ops.norm_rope_gradients(operands, cos, sin, positions, eps, interleaved)
         dx = [None if r is None else PolyTensor.from_stacked(r[0]) for r in results]
         dw = [None if r is None or r[1] is None else PolyTensor.from_stacked(r[1]) for r in results]
         return (*dx, *dw, None, None, None, None, None)
@@ -145,8 +147,7 @@ def qk_norm_rope(query, key, cos, sin, positions=None, query_weight=None, key_we
         raise NotImplementedError(f"qk_norm_rope: {reason}")
     cos, sin, eps, interleaved = cos.contiguous(), sin.contiguous(), float(eps), bool(interleaved)
     if positions is not None:
-        positions = positions.reshape(-1) if positions.shape[0] == 1 or positions.ndim == 1 else positions
-        positions = positions.contiguous()
+        positions = (positions.reshape(-1) if positions.ndim == 2 and positions.shape[0] == 1 else positions).contiguous()
     degree = next(x.degree for x in (query, key, query_weight, key_weight) if isinstance(x, PolyTensor))
     if not isinstance(query, PolyTensor) and isinstance(query_weight, PolyTensor):
         query = PolyTensor.constant(query, degree)

@@ -777,66 +777,17 @@ torch.library.register_autograd(f"{NAMESPACE}::series_binary", _binary_backward,
 torch.library.register_autograd(f"{NAMESPACE}::series_binary_orders", _binary_backward, setup_context=_binary_setup)
 
 
-def _dropout_setup(ctx, inputs, output):
-    x, seed, p = inputs
-    ctx.save_for_backward(seed)
-    ctx.meta = (len(x), p)
+# (dropout_series_orders, norm_rope_series_orders and token_log_probs_series record their coefficient gradients in
+# C++, csrc/torch_ops.cpp, by the same rule)
 
-
-def _dropout_backward(ctx, grad):
-    # the mask acts on each order alone: the cotangents' dropout, order by order (differentiable again)
-    (seed,) = ctx.saved_tensors
-    n, p = ctx.meta
-    cots = _reversed(grad)[::-1]
-    return _returned(ctx, list(dropout_series_orders(cots, seed, p)))
-
-
-torch.library.register_autograd(f"{NAMESPACE}::dropout_series", _dropout_backward, setup_context=_dropout_setup)
-torch.library.register_autograd(f"{NAMESPACE}::dropout_series_orders", _dropout_backward, setup_context=_dropout_setup)
-
-
-def _norm_rope_setup(ctx, inputs, output):
-    q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved = inputs
-    ctx.save_for_backward(*q, *k, *q_weight, *k_weight, cos, sin, *([] if positions is None else [positions]))
-    ctx.meta = (len(q), len(k), len(q_weight), len(k_weight), eps, interleaved, _grads_flag(q_weight), _grads_flag(k_weight))
-
-
-def _norm_rope_backward(ctx, *grads):
-    _once("qk_norm_rope")
-    nq, nk, nqw, nkw, eps, interleaved, need_qw, need_kw = ctx.meta
-    saved = list(ctx.saved_tensors)
-    take = lambda n: [saved.pop(0) for _ in range(n)]   # noqa: E731
-    q, k, qw, kw = take(nq), take(nk), take(nqw), take(nkw)
-    cos, sin = take(2)
-    positions = saved[0] if saved else None
-    if len(grads) == 1:   # the tensor-per-order form
-        gq, gk = list(grads[0][:nq]), list(grads[0][nq:])
-    else:
-        gq, gk = (None if g is None else list(g.unbind(0)) for g in grads)
-    results = norm_rope_gradients([(q, gq, qw, need_qw), (k, gk, kw, need_kw)], cos, sin, positions, eps, interleaved,
-                                  reverse=True)
-    dx, dw = [], []
-    for (x, w, got) in ((q, qw, results[0]), (k, kw, results[1])):
-        dx.append([None] * len(x) if got is None or got[0] is None else _read_back(got[0], len(x)))
-        if got is None or got[1] is None:
-            dw.append([None] * len(w))
-        else:   # an ordinary weight's is the last order of the gradient series
-            dw.append([got[1][0]] if len(w) == 1 else _read_back(got[1], len(w)))
-    return _returned(ctx, dx[0], dx[1], None, None, None, dw[0], dw[1])
-
-
-def norm_rope_gradients(operands, cos, sin, positions, eps, interleaved, reverse):
-    """(dx, dw) gradient series of each operand (coefficients, cotangents, weight coefficients, whether the
-    weight's gradient is wanted): None for an operand without orders or cotangents. ``reverse``: the
-    cotangents are those of coefficient autograd, which the kernel takes in reverse order; an ordinary
-    weight's gradient is then one order, otherwise (a gradient series) a weight's has all."""
+def norm_rope_gradients(operands, cos, sin, positions, eps, interleaved):
+    """(dx, dw) gradient series of each operand (coefficients, cotangent series, weight coefficients, whether the
+    weight's gradient is wanted): None for an operand without orders or cotangents."""
     calls, slots = [], []
     for i, (x, g, w, need) in enumerate(operands):
         if not x or g is None or all(c is None for c in g):
             continue
-        cots = _reversed(g)
-        want = 0 if not (need and w) else (1 if reverse and len(w) == 1 else len(x))
-        calls.append((x, cots if reverse else cots[::-1], w, want))
+        calls.append((x, _reversed(g)[::-1], w, len(x) if need and w else 0))
         slots.append(i)
     results = [None] * len(operands)
     if not calls:
@@ -847,34 +798,6 @@ def norm_rope_gradients(operands, cos, sin, positions, eps, interleaved, reverse
     for j, i in enumerate(slots):
         results[i] = (out[j], out[2 + j] if calls[j][3] else None)
     return results
-
-
-torch.library.register_autograd(f"{NAMESPACE}::norm_rope_series", _norm_rope_backward, setup_context=_norm_rope_setup)
-torch.library.register_autograd(f"{NAMESPACE}::norm_rope_series_orders", _norm_rope_backward,
-                                setup_context=_norm_rope_setup)
-
-
-def _log_probs_setup(ctx, inputs, output):
-    z, tokens, ignore_index, softcap, top = inputs
-    log_probs, entropy, top_tokens, top_log_probs, lse = output
-    ctx.mark_non_differentiable(top_tokens, lse)
-    ctx.save_for_backward(*z, tokens, entropy, top_tokens, lse)
-    ctx.meta = (len(z), ignore_index, softcap, top)
-
-
-def _log_probs_backward(ctx, grad_log_probs, grad_entropy, grad_tokens, grad_top, grad_lse):
-    _once("token_log_probs")
-    n, ignore_index, softcap, top = ctx.meta
-    saved = ctx.saved_tensors
-    z, (tokens, entropy, top_tokens, lse) = list(saved[:n]), saved[n:]
-    cots = [[] if g is None or (i == 2 and top == 0) else [c.contiguous() for c in g.to(lse.dtype).flip(0).unbind(0)]
-            for i, g in enumerate((grad_log_probs, grad_entropy, grad_top))]
-    dz = token_log_probs_series_backward(z, tokens, ignore_index, softcap, lse, entropy, top_tokens, *cots)
-    return _returned(ctx, _read_back(dz, n))
-
-
-torch.library.register_autograd(f"{NAMESPACE}::token_log_probs_series", _log_probs_backward,
-                                setup_context=_log_probs_setup)
 
 
 # The complex-direction plumbing is linear in its inputs. Its gradients follow torch's

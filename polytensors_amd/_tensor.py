@@ -304,7 +304,8 @@ class PolyTensor(torch.Tensor):
         """
         from ._fused_norm_rope import qk_norm_rope
 
-        return qk_norm_rope(query, key, cos, sin, positions, query_weight, key_weight, eps, interleaved)
+        with torch._C.DisableTorchFunctionSubclass():   # (as in __torch_function__'s routed paths)
+            return qk_norm_rope(query, key, cos, sin, positions, query_weight, key_weight, eps, interleaved)
 
     @staticmethod
     def token_log_probs(logits, tokens, top=0, softcap=None, ignore_index=-100):
@@ -318,7 +319,8 @@ class PolyTensor(torch.Tensor):
         """
         from ._fused_log_probs import token_log_probs
 
-        return token_log_probs(logits, tokens, top=top, softcap=softcap, ignore_index=ignore_index)
+        with torch._C.DisableTorchFunctionSubclass():
+            return token_log_probs(logits, tokens, top=top, softcap=softcap, ignore_index=ignore_index)
 
     @staticmethod
     def dropout(input, p=0.5, seed=None):
@@ -331,7 +333,8 @@ class PolyTensor(torch.Tensor):
         """
         from ._fused_dropout import dropout
 
-        return dropout(input, p, seed)
+        with torch._C.DisableTorchFunctionSubclass():
+            return dropout(input, p, seed)
 
     def backward(self, gradient=None, retain_graph=None, create_graph=False, inputs=None):
         """Reverse mode through the series (/root/reference/src/polytensors/_tensor.py:325-338).

@@ -1,9 +1,9 @@
 // Log probabilities of given tokens, the entropy and the most probable alternatives of rows of logits,
 // as degree-K series, in one streaming pass a row.
 //
-// For a row z(t) over C classes, with m = max z_0 and the row's series shifted by (m, rho_1, .., rho_K),
-// rho the given token's (a shift common to all classes changes no probability, and no order then loses
-// its digits to one):
+// For a row z(t) over C classes, with m = max z_0 and the row's series shifted by (m, rho_1, .., rho_K), rho
+// the mean of the row's first 64 classes (any shift common to all classes changes no probability; this
+// one leaves values of the size of their spread, so that no order loses its digits to an offset):
 //   E = exp(z) a class,   F_k = k E_k = sum_{j=1..k} j z_j E_{k-j}
 //   S = sum E,   Q = sum E (*) z,   k Q_k = sum_c (F_k + sum_{a=1..k} F_a z_{k-a})
 //   L = log S (the log series),  log p = z - L,   H = L - Q / S  (= -sum p (*) log p)
@@ -150,35 +150,42 @@ struct LpKernelArgs {
   int top;
   MPtrs<A> log_probs, entropy, top_log_probs, lse;
   int64_t* top_tokens;
-  A* partial;                       // [row][split][2 K + 3]
+  A* partial;                       // [row][split][3 K + 3]: m, S, W and the shift, the same in every piece
   typename TopKey<A>::U* key_bits;  // [row][split][top]
   uint32_t* key_class;
 };
 
-// The given token's series (zero where it is no class) and the shift of the higher orders.
+// The shift of the row's higher orders, by every wave alike: the mean of its first 64 classes, of the finite
+// values among them.
 template <typename T, int K, bool CAP>
-__device__ __forceinline__ bool lp_token(const LpKernelArgs<T>& a, int64_t row, int64_t y, typename AccOf<T>::type (&zy)[K + 1],
-                                         typename AccOf<T>::type (&rho)[K + 1]) {
+__device__ __forceinline__ void lp_shift(const LpKernelArgs<T>& a, int64_t row, typename AccOf<T>::type (&rho)[K + 1]) {
   using A = typename AccOf<T>::type;
-  const bool valid = y >= 0 && y < a.classes;
+  const int n = a.classes < kWave ? static_cast<int>(a.classes) : kWave, lane = threadIdx.x % kWave;
+  A x[K + 1];
 #pragma unroll
-  for (int k = 0; k <= K; ++k) zy[k] = valid ? to_acc(a.z.p[k][row * a.row_stride + y]) : A(0);
-  if constexpr (CAP) softcap_series<A, K>(zy, a.cap, a.inv_cap);
+  for (int k = CAP ? 0 : 1; k <= K; ++k) x[k] = to_acc(a.z.p[k][row * a.row_stride + (lane < n ? lane : 0)]);
+  if constexpr (CAP) softcap_series<A, K>(x, a.cap, a.inv_cap);
   rho[0] = A(0);
 #pragma unroll
-  for (int k = 1; k <= K; ++k) rho[k] = valid && fabs(zy[k]) < A(__builtin_huge_val()) ? zy[k] : A(0);
-  return valid;
+  for (int k = 1; k <= K; ++k) {
+    const A sum = wave_sum(lane < n && fabs(x[k]) < A(__builtin_huge_val()) ? x[k] : A(0)) / A(n);
+    rho[k] = fabs(sum) < A(__builtin_huge_val()) ? sum : A(0);
+  }
 }
 
 // Results of a row from its whole state, by the block: thread 0 the series, then a thread an alternative.
 template <typename T, int K, bool CAP, bool TOP>
 __device__ __forceinline__ void lp_finish(const LpKernelArgs<T>& a, int64_t row, int64_t y,
                                           const LpState<typename AccOf<T>::type, K>& st,
+                                          const typename AccOf<T>::type (&rho)[K + 1],
                                           const TopKey<typename AccOf<T>::type>* best, typename AccOf<T>::type* shared) {
   using A = typename AccOf<T>::type;
-  A zy[K + 1], rho[K + 1];
-  const bool valid = lp_token<T, K, CAP>(a, row, y, zy, rho);
   if (threadIdx.x == 0) {
+    const bool valid = y >= 0 && y < a.classes;
+    A zy[K + 1];
+#pragma unroll
+    for (int k = 0; k <= K; ++k) zy[k] = valid ? to_acc(a.z.p[k][row * a.row_stride + y]) : A(0);
+    if constexpr (CAP) softcap_series<A, K>(zy, a.cap, a.inv_cap);
     A n[K + 1], L[K + 1], Q[K + 1];
     n[0] = A(1);
     const A inv = A(1) / st.S[0];
@@ -257,20 +264,16 @@ struct LpTopShared {
   int n_threads, n_found;
 };
 
-// The block's `top` first classes of z0[0 .. n), whose vectors start at `head`; classes are numbered from `first`.
-template <typename T>
-__device__ void lp_select(const T* z0, int64_t n, int64_t head, uint32_t first, TopKey<typename AccOf<T>::type> own, bool careful,
-                          int top, LpTopShared<typename AccOf<T>::type>& sh) {
-  using A = typename AccOf<T>::type;
-  constexpr int V = VecWidth<T>::value;
-  const int64_t nvec = (n - head) / V, around = n - nvec * V;
-  TopKey<A> g = own;
+// A key that at least `top` of the threads' own reach, a little below the top-th: the top-th largest of 64
+// groups' maxima (no key's where fewer groups have one). The counters are cleared.
+template <typename A, typename Shared>
+__device__ __forceinline__ TopKey<A> lp_bound(TopKey<A> own, int top, Shared& sh) {
 #pragma unroll
   for (int mask = 1; mask <= 2; mask <<= 1) {
-    const TopKey<A> o = shuffled(g, mask);
-    if (before(o, g)) g = o;
+    const TopKey<A> o = shuffled(own, mask);
+    if (before(o, own)) own = o;
   }
-  if (threadIdx.x % 4 == 0) sh.group[threadIdx.x / 4] = g;
+  if (threadIdx.x % 4 == 0) sh.group[threadIdx.x / 4] = own;
   if (threadIdx.x == 0) {
     sh.bound = no_key<A>();
     sh.n_threads = sh.n_found = 0;
@@ -279,11 +282,22 @@ __device__ void lp_select(const T* z0, int64_t n, int64_t head, uint32_t first, 
   if (threadIdx.x < 64) {
     const TopKey<A> key = sh.group[threadIdx.x];
     int place = 0;
+#pragma unroll 16
     for (int j = 0; j < 64; ++j) place += before(sh.group[j], key);
     if (place == top - 1 && key.v != 0) sh.bound = key;
   }
   __syncthreads();
-  const TopKey<A> bound = sh.bound;
+  return sh.bound;
+}
+
+// The block's `top` first classes of z0[0 .. n), whose vectors start at `head`; classes are numbered from `first`.
+template <typename T>
+__device__ void lp_select(const T* z0, int64_t n, int64_t head, uint32_t first, TopKey<typename AccOf<T>::type> own, bool careful,
+                          int top, LpTopShared<typename AccOf<T>::type>& sh) {
+  using A = typename AccOf<T>::type;
+  constexpr int V = VecWidth<T>::value;
+  const int64_t nvec = (n - head) / V, around = n - nvec * V;
+  const TopKey<A> bound = lp_bound(own, top, sh);
   bool done = false;
   if (bound.v != 0 && !careful) {
     if (!before(bound, own)) sh.threads[atomicAdd(&sh.n_threads, 1)] = threadIdx.x;
@@ -374,8 +388,8 @@ __global__ __launch_bounds__(kLpThreads) void token_log_probs_series_kernel(cons
   const int64_t c0 = split * a.piece < a.classes ? split * a.piece : a.classes;
   const int64_t n = c0 + a.piece < a.classes ? a.piece : a.classes - c0;
   const int64_t base = row * a.row_stride + c0;
-  A zy[K + 1], rho[K + 1];
-  lp_token<T, K, CAP>(a, row, y, zy, rho);
+  A rho[K + 1];
+  lp_shift<T, K, CAP>(a, row, rho);
 
   LpState<A, K> st;
   lp_clear(st);
@@ -489,7 +503,7 @@ __global__ __launch_bounds__(kLpThreads) void token_log_probs_series_kernel(cons
     // (S_0 is no number where a logit is none, which a thread's maximum does not show)
     lp_select<T>(a.z.p[0] + base, n, head, static_cast<uint32_t>(c0), own, st.S[0] != st.S[0], a.top, sh);
     if (a.splits == 1) {
-      lp_finish<T, K, CAP, true>(a, row, y, st, sh.best, series);
+      lp_finish<T, K, CAP, true>(a, row, y, st, rho, sh.best, series);
     } else {
       const int64_t at = static_cast<int64_t>(blockIdx.x) * a.top + threadIdx.x;
       if (static_cast<int>(threadIdx.x) < a.top) {
@@ -498,21 +512,29 @@ __global__ __launch_bounds__(kLpThreads) void token_log_probs_series_kernel(cons
       }
     }
   } else if (a.splits == 1) {
-    lp_finish<T, K, CAP, false>(a, row, y, st, nullptr, series);
+    lp_finish<T, K, CAP, false>(a, row, y, st, rho, nullptr, series);
   }
   if (a.splits > 1 && threadIdx.x == 0) {
-    A* out = a.partial + static_cast<int64_t>(blockIdx.x) * (2 * K + 3);
+    A* out = a.partial + static_cast<int64_t>(blockIdx.x) * (3 * K + 3);
     out[0] = st.m;
 #pragma unroll
     for (int k = 0; k <= K; ++k) {
       out[1 + k] = st.S[k];
       out[2 + K + k] = st.W[k];
+      if (k > 0) out[2 + 2 * K + k] = rho[k];
     }
   }
 }
 
-// A row's pieces joined: a lane of every wave takes a piece's state; the pieces' alternatives that reach the
-// largest of the pieces' last ones (which `top` classes reach) are ranked.
+template <typename A>
+struct LpJoinShared {
+  TopKey<A> group[64], bound, best[kLpMaxTop], found[kLpMaxSplits * kLpMaxTop];
+  int n_threads, n_found;
+};
+
+// A row's pieces joined: a lane of every wave takes a piece's state; of the pieces' alternatives those that reach
+// the bound of the threads' largest are ranked. (Ranking all 64 x 20 of 8 rows that reached the largest of the
+// pieces' last ones, about half of them: 82 us.)
 template <typename T, int K, bool CAP, bool TOP>
 __global__ __launch_bounds__(kLpThreads) void token_log_probs_join_kernel(const LpKernelArgs<T> a) {
   using A = typename AccOf<T>::type;
@@ -525,9 +547,10 @@ __global__ __launch_bounds__(kLpThreads) void token_log_probs_join_kernel(const 
   }
   LpState<A, K> st;
   lp_clear(st);
+  A rho[K + 1];
   const uint32_t lane = threadIdx.x % kWave;
+  const A* in = a.partial + (row * a.splits + (lane < a.splits ? lane : 0)) * (3 * K + 3);
   if (lane < a.splits) {
-    const A* in = a.partial + (row * a.splits + lane) * (2 * K + 3);
     st.m = in[0];
 #pragma unroll
     for (int k = 0; k <= K; ++k) {
@@ -535,29 +558,32 @@ __global__ __launch_bounds__(kLpThreads) void token_log_probs_join_kernel(const 
       st.W[k] = in[2 + K + k];
     }
   }
+  rho[0] = A(0);
+#pragma unroll
+  for (int k = 1; k <= K; ++k) rho[k] = in[2 + 2 * K + k];
   lp_join_wave(st);
   if constexpr (TOP) {
-    __shared__ TopKey<A> found[kLpMaxSplits * kLpMaxTop], best[kLpMaxTop];
-    __shared__ int n_found;
+    __shared__ LpJoinShared<A> sh;
     const auto* bits = a.key_bits + row * a.splits * a.top;
     const uint32_t* classes = a.key_class + row * a.splits * a.top;
-    TopKey<A> bound = lane < a.splits ? TopKey<A>{bits[lane * a.top + a.top - 1], classes[lane * a.top + a.top - 1]} : no_key<A>();
+    const int n = static_cast<int>(a.splits) * a.top;
+    constexpr int kEach = kLpMaxSplits * kLpMaxTop / kLpThreads;
+    TopKey<A> mine[kEach], own = no_key<A>();
 #pragma unroll
-    for (int mask = 1; mask < kWave; mask <<= 1) {
-      const TopKey<A> o = shuffled(bound, mask);
-      if (before(o, bound)) bound = o;
+    for (int i = 0; i < kEach; ++i) {
+      const int at = threadIdx.x + i * kLpThreads;
+      mine[i] = at < n ? TopKey<A>{bits[at], classes[at]} : no_key<A>();
+      if (before(mine[i], own)) own = mine[i];
     }
-    if (threadIdx.x == 0) n_found = 0;
+    const TopKey<A> bound = lp_bound(own, a.top, sh);   // (none: every key is ranked)
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (mine[i].v != 0 && !before(bound, mine[i])) sh.found[atomicAdd(&sh.n_found, 1)] = mine[i];
     __syncthreads();
-    for (int i = threadIdx.x; i < static_cast<int>(a.splits) * a.top; i += kLpThreads) {
-      const TopKey<A> key{bits[i], classes[i]};
-      if (key.v != 0 && !before(bound, key)) found[atomicAdd(&n_found, 1)] = key;
-    }
-    __syncthreads();
-    lp_rank(found, n_found, a.top, best);
-    lp_finish<T, K, CAP, true>(a, row, y, st, best, series);
+    lp_rank(sh.found, sh.n_found, a.top, sh.best);
+    lp_finish<T, K, CAP, true>(a, row, y, st, rho, sh.best, series);
   } else {
-    lp_finish<T, K, CAP, false>(a, row, y, st, nullptr, series);
+    lp_finish<T, K, CAP, false>(a, row, y, st, rho, nullptr, series);
   }
 }
 
@@ -590,7 +616,7 @@ static int launch_log_probs_k(const LogProbArgs& in) {
     a.key_bits = reinterpret_cast<typename TopKey<A>::U*>(w);
     w += sizeof(A) * in.rows * splits * in.top;
     a.partial = reinterpret_cast<A*>(w);
-    w += sizeof(A) * in.rows * splits * (2 * K + 3);
+    w += sizeof(A) * in.rows * splits * (3 * K + 3);
     a.key_class = reinterpret_cast<uint32_t*>(w);
   }
   const dim3 grid(static_cast<uint32_t>(in.rows * splits)), block(kLpThreads);

@@ -15,7 +15,7 @@ size_t log_prob_workspace(int degree, int64_t rows, int64_t classes, int top, in
   const int64_t splits = log_prob_splits(rows, classes, elem_size);
   if (splits == 1) return 0;
   const size_t acc = elem_size == 8 ? 8 : 4;
-  return static_cast<size_t>(rows * splits) * (acc * (top + 2 * degree + 3) + sizeof(uint32_t) * top);
+  return static_cast<size_t>(rows * splits) * (acc * (top + 3 * degree + 3) + sizeof(uint32_t) * top);
 }
 
 }  // namespace pt

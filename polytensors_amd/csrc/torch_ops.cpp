@@ -5,11 +5,15 @@
 // passes the K+1 coefficient pointers of every series as they are stored (no
 // stacking copies) and launches on the current HIP stream of the operands'
 // device; a non-zero status becomes RuntimeError with pt_last_error(). The
-// fake (shape) and autograd registrations of these operators are made from
-// Python (polytensors_amd/_ops.py).
+// fake (shape) registrations of these operators are made from Python
+// (polytensors_amd/_ops.py), and so are the autograd registrations but those of
+// dropout, the per-head norm and rotation and the token log probabilities, which
+// are here: recorded in Python, forward and gradient of one training step of the
+// rotation took 290 us of host time, longer than its kernels.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <array>
@@ -1077,6 +1081,195 @@ Tensor token_log_probs_series_backward(const TensorList& z, const Tensor& tokens
   return out;
 }
 
+// ---- Coefficient-level autograd of the three above ------------------------------------
+//
+// As polytensors_amd/_ops.py describes it: the gradients of input coefficients are the gradient series
+// of the reversed cotangents, read in reverse.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// An operator of this library through the dispatcher (fake tensors take their own implementations there),
+// with its implementation's signature.
+template <typename F>
+auto dispatched(const char* name, F*) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+
+void refuse_second_order(const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::GradMode::is_enabled(), what,
+                              ": second-order coefficient autograd through the fused kernels is not implemented");
+}
+
+// Cotangents [from, from + n) as contiguous tensors, in reverse order; empty where none is given.
+TensorList reversed_cotangents(const variable_list& grads, size_t from, size_t n) {
+  const Tensor* any = nullptr;
+  for (size_t i = 0; i < n; ++i)
+    if (grads[from + i].defined()) any = &grads[from + i];
+  TensorList out;
+  if (any == nullptr) return out;
+  for (size_t i = n; i-- > 0;)
+    out.push_back(grads[from + i].defined() ? grads[from + i].contiguous() : at::zeros_like(*any, at::MemoryFormat::Contiguous));
+  return out;
+}
+
+// The orders of a stacked cotangent, in reverse; empty where it is undefined.
+TensorList reversed_orders(const Tensor& grad, at::ScalarType dtype) {
+  TensorList out;
+  if (!grad.defined()) return out;
+  const Tensor g = grad.to(dtype);
+  for (int64_t i = g.size(0); i-- > 0;) out.push_back(g.select(0, i).contiguous());
+  return out;
+}
+
+bool any_requires_grad(at::TensorList ts) {
+  for (const Tensor& t : ts)
+    if (t.requires_grad()) return true;
+  return false;
+}
+
+struct NormRopeFunction : public torch::autograd::Function<NormRopeFunction> {
+  static variable_list forward(AutogradContext* ctx, at::TensorList q, at::TensorList k, const Tensor& cos, const Tensor& sin,
+                               const c10::optional<Tensor>& positions, at::TensorList q_weight, at::TensorList k_weight,
+                               double eps, bool interleaved) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    variable_list saved;
+    for (at::TensorList ts : {q, k, q_weight, k_weight}) saved.insert(saved.end(), ts.begin(), ts.end());
+    saved.push_back(cos);
+    saved.push_back(sin);
+    if (positions) saved.push_back(*positions);
+    ctx->save_for_backward(saved);
+    ctx->saved_data["sizes"] = std::vector<int64_t>{static_cast<int64_t>(q.size()), static_cast<int64_t>(k.size()),
+                                                    static_cast<int64_t>(q_weight.size()), static_cast<int64_t>(k_weight.size()),
+                                                    any_requires_grad(q_weight), any_requires_grad(k_weight)};
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->set_materialize_grads(false);
+    static const auto op = dispatched("polytensors_amd::norm_rope_series_orders", &norm_rope_series_orders);
+    return op.call(q.vec(), k.vec(), cos, sin, positions, q_weight.vec(), k_weight.vec(), eps, interleaved);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_second_order("qk_norm_rope");
+    const auto n = ctx->saved_data["sizes"].toIntVector();
+    const variable_list saved = ctx->get_saved_variables();
+    size_t at = 0;
+    auto take = [&](int64_t count) {
+      TensorList out(saved.begin() + at, saved.begin() + at + count);
+      at += count;
+      return out;
+    };
+    TensorList x[2] = {take(n[0]), take(n[1])};
+    TensorList w[2] = {take(n[2]), take(n[3])};
+    const Tensor cos = saved[at], sin = saved[at + 1];
+    c10::optional<Tensor> positions;
+    if (saved.size() > at + 2) positions = saved[at + 2];
+    TensorList g[2] = {reversed_cotangents(grads, 0, n[0]), reversed_cotangents(grads, n[0], n[1])};
+    // an operand without cotangents is left out of the call
+    const int first = g[0].empty() ? 1 : 0, last = g[1].empty() ? 0 : 1;
+    variable_list result(n[0] + n[1] + 3 + n[2] + n[3] + 2);
+    if (first > last) return result;
+    // an ordinary weight's gradient is the last order of the series alone
+    auto want = [&](int o) { return n[4 + o] == 0 ? int64_t{0} : n[2 + o] == 1 ? int64_t{1} : n[o]; };
+    const TensorList none;
+    const bool both = last > first;
+    static const auto op = dispatched("polytensors_amd::norm_rope_series_backward", &norm_rope_series_backward);
+    auto got = op.call(x[first], both ? x[1] : none, g[first], both ? g[1] : none, cos, sin, positions, w[first],
+                       both ? w[1] : none, ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool(),
+                       want(first), both ? want(1) : 0);
+    for (int o = first; o <= last; ++o) {
+      const bool slot = both && o == 1;
+      const Tensor& dx = slot ? std::get<1>(got) : std::get<0>(got);
+      const Tensor& dw = slot ? std::get<3>(got) : std::get<2>(got);
+      const int64_t at_x = o == 0 ? 0 : n[0], at_w = n[0] + n[1] + 3 + (o == 0 ? 0 : n[2]);
+      for (int64_t i = 0; i < n[o]; ++i) result[at_x + i] = dx.select(0, n[o] - 1 - i);
+      if (want(o) > 0)
+        for (int64_t i = 0; i < n[2 + o]; ++i) result[at_w + i] = dw.select(0, n[2 + o] - 1 - i);
+    }
+    return result;
+  }
+};
+
+TensorList norm_rope_series_orders_autograd(const TensorList& q, const TensorList& k, const Tensor& cos, const Tensor& sin,
+                                            const c10::optional<Tensor>& positions, const TensorList& q_weight,
+                                            const TensorList& k_weight, double eps, bool interleaved) {
+  return NormRopeFunction::apply(at::TensorList(q), at::TensorList(k), cos, sin, positions, at::TensorList(q_weight),
+                                 at::TensorList(k_weight), eps, interleaved);
+}
+
+struct LogProbsFunction : public torch::autograd::Function<LogProbsFunction> {
+  static variable_list forward(AutogradContext* ctx, at::TensorList z, const Tensor& tokens, int64_t ignore_index, double softcap,
+                               int64_t top) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static const auto op = dispatched("polytensors_amd::token_log_probs_series", &token_log_probs_series);
+    auto [log_probs, entropy, top_tokens, top_log_probs, lse] = op.call(z.vec(), tokens, ignore_index, softcap, top);
+    variable_list saved(z.begin(), z.end());
+    // (the entropy is an output: a copy, so that a caller may change it)
+    for (const Tensor& t : {tokens, entropy.clone(), top_tokens, lse}) saved.push_back(t);
+    ctx->save_for_backward(saved);
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["softcap"] = softcap;
+    ctx->saved_data["top"] = top;
+    ctx->mark_non_differentiable({top_tokens, lse});
+    ctx->set_materialize_grads(false);
+    return {log_probs, entropy, top_tokens, top_log_probs, lse};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_second_order("token_log_probs");
+    const variable_list saved = ctx->get_saved_variables();
+    const size_t n = saved.size() - 4;
+    const TensorList z(saved.begin(), saved.begin() + n);
+    variable_list result(n + 4);
+    const at::ScalarType acc = acc_type(z[0].scalar_type());
+    TensorList cot_top;
+    if (ctx->saved_data["top"].toInt() > 0) cot_top = reversed_orders(grads[3], acc);
+    static const auto op = dispatched("polytensors_amd::token_log_probs_series_backward", &token_log_probs_series_backward);
+    const Tensor dz = op.call(
+        z, saved[n], ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["softcap"].toDouble(), saved[n + 3], saved[n + 1],
+        saved[n + 2], reversed_orders(grads[0], acc), reversed_orders(grads[1], acc), cot_top);
+    for (size_t i = 0; i < n; ++i) result[i] = dz.select(0, static_cast<int64_t>(n - 1 - i));
+    return result;
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_log_probs_series_autograd(const TensorList& z, const Tensor& tokens,
+                                                                                   int64_t ignore_index, double softcap,
+                                                                                   int64_t top) {
+  const variable_list y = LogProbsFunction::apply(at::TensorList(z), tokens, ignore_index, softcap, top);
+  return {y[0], y[1], y[2], y[3], y[4]};
+}
+
+// The mask acts on each order alone: the cotangents' dropout, order by order (recorded again for further derivatives).
+struct DropoutFunction : public torch::autograd::Function<DropoutFunction> {
+  static variable_list forward(AutogradContext* ctx, at::TensorList x, const Tensor& seed, double p) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    ctx->save_for_backward({seed});
+    ctx->saved_data["p"] = p;
+    ctx->set_materialize_grads(false);
+    static const auto op = dispatched("polytensors_amd::dropout_series_orders", &dropout_series_orders);
+    return op.call(x.vec(), seed, p);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    static const auto op = dispatched("polytensors_amd::dropout_series_orders", &dropout_series_orders);
+    const Tensor seed = ctx->get_saved_variables()[0];
+    variable_list result(grads.size() + 2);
+    TensorList cots;
+    for (const Tensor& g : grads)
+      if (g.defined()) cots.push_back(g.contiguous());
+    if (cots.empty()) return result;
+    const TensorList dx = op.call(cots, seed, ctx->saved_data["p"].toDouble());
+    for (size_t i = 0, j = 0; i < grads.size(); ++i)
+      if (grads[i].defined()) result[i] = dx[j++];
+    return result;
+  }
+};
+
+TensorList dropout_series_orders_autograd(const TensorList& x, const Tensor& seed, double p) {
+  return DropoutFunction::apply(at::TensorList(x), seed, p);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(polytensors_amd, m) {
@@ -1146,4 +1339,10 @@ TORCH_LIBRARY_IMPL(polytensors_amd, CUDA, m) {
   m.impl("norm_rope_series_backward", &norm_rope_series_backward);
   m.impl("token_log_probs_series", &token_log_probs_series);
   m.impl("token_log_probs_series_backward", &token_log_probs_series_backward);
+}
+
+TORCH_LIBRARY_IMPL(polytensors_amd, Autograd, m) {
+  m.impl("norm_rope_series_orders", &norm_rope_series_orders_autograd);
+  m.impl("token_log_probs_series", &token_log_probs_series_autograd);
+  m.impl("dropout_series_orders", &dropout_series_orders_autograd);
 }

@@ -96,7 +96,7 @@ def test_log_probs_workspace():
     size = _lib.load().pt_token_log_probs_series_workspace_size
     assert size(0, 2, 4096, 32000, 5) == 0 and size(0, 2, 4, 500, 5) == 0     # rows enough, or too short to cut
     few = size(0, 2, 4, 1 << 17, 5)                                           # 64 pieces a row
-    assert few == 4 * 64 * (4 * (5 + 7) + 4 * 5)
+    assert few == 4 * 64 * (4 * (5 + 9) + 4 * 5)
     assert size(0, 9, 4, 1 << 17, 5) == 0 and size(0, 2, 4, 1 << 17, 33) == 0
 
 
