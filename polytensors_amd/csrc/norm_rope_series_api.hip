@@ -1,12 +1,6 @@
 // C ABI of the per-head norm and rotation kernels.
 #include "norm_rope_series.h"
 
-namespace pt {
-
-int64_t norm_rope_partials(int64_t rows) { return rows < 1024 ? rows : 1024; }
-
-}  // namespace pt
-
 namespace {
 
 int check(const char* what, const pt::NormRopeArgs& a, int dtype, bool backward) {
