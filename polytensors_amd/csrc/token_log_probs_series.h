@@ -48,7 +48,7 @@ template <typename T>
 int launch_log_probs_bwd(const LogProbBwdArgs& a);
 
 // Pieces that a row is cut into so that few rows fill the device, and the bytes of their partial results.
-int64_t log_prob_splits(int64_t rows, int64_t classes, int elem_size);
+int64_t log_prob_splits(int64_t rows, int64_t classes, int elem_size, bool backward);
 size_t log_prob_workspace(int degree, int64_t rows, int64_t classes, int top, int elem_size);
 
 }  // namespace pt

@@ -72,6 +72,18 @@ __device__ __forceinline__ TopKey<A> shuffled(const TopKey<A>& k, int mask) {
           static_cast<uint32_t>(__shfl_xor(static_cast<int>(k.i), mask, kWave))};
 }
 
+// Elements before the vectors of a row, which start at the first cache line that begins at or after p, so that a wave's
+// accesses take whole lines; in rows below 16 KB, where the elements before them would cost more, at the first 16
+// bytes (4096 x 32001 bfloat16, degree 3: 178 and 490 us forward and backward from the first 16 bytes, 168 and 418 from the
+// first line; 16384 x 1000 float32, degree 2: 101 and 84, 108 and 87).
+template <typename T>
+__device__ __forceinline__ int64_t lp_head(const T* p, int64_t n) {
+  const uint32_t line = n * static_cast<int64_t>(sizeof(T)) >= 16384 ? 128u : 16u;
+  const int64_t head = static_cast<int64_t>((0u - static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p))) & (line - 1)) /
+                       static_cast<int64_t>(sizeof(T));
+  return head < n ? head : n;
+}
+
 // ---- a row's running state ----------------------------------------------------
 template <typename A, int K>
 struct LpState {
@@ -381,6 +393,8 @@ __global__ __launch_bounds__(kLpThreads) void token_log_probs_series_kernel(cons
   const uint32_t split = blockIdx.x % a.splits;
   const int64_t row = blockIdx.x / a.splits;
   const int64_t y = a.tokens[row];
+  A rho[K + 1];
+  lp_shift<T, K, CAP>(a, row, rho);   // (its loads beside the token's, not after it)
   if (y == a.ignore_index) {
     if (a.splits == 1) lp_ignored<T, K, TOP>(a, row);
     return;
@@ -388,9 +402,6 @@ __global__ __launch_bounds__(kLpThreads) void token_log_probs_series_kernel(cons
   const int64_t c0 = split * a.piece < a.classes ? split * a.piece : a.classes;
   const int64_t n = c0 + a.piece < a.classes ? a.piece : a.classes - c0;
   const int64_t base = row * a.row_stride + c0;
-  A rho[K + 1];
-  lp_shift<T, K, CAP>(a, row, rho);
-
   LpState<A, K> st;
   lp_clear(st);
   A raw_max = kNegInf;   // the maximum before the softcap
@@ -442,7 +453,7 @@ __global__ __launch_bounds__(kLpThreads) void token_log_probs_series_kernel(cons
   };
 
   constexpr int U = 2;
-  const int64_t head = ce_head(a.z.p[0] + base, n), nvec = (n - head) / V;
+  const int64_t head = lp_head(a.z.p[0] + base, n), nvec = (n - head) / V;
   int64_t j = threadIdx.x;
   for (; j + (U - 1) * kLpThreads < nvec; j += U * kLpThreads) {
     Vec<T, V> v[U][K + 1];
@@ -599,7 +610,7 @@ static int launch_log_probs_k(const LogProbArgs& in) {
     a.lse.p[k] = static_cast<A*>(in.lse[k]);
     if (in.top > 0) a.top_log_probs.p[k] = static_cast<A*>(in.top_log_probs[k]);
   }
-  const int64_t splits = log_prob_splits(in.rows, in.classes, sizeof(T));
+  const int64_t splits = log_prob_splits(in.rows, in.classes, sizeof(T), false);
   a.classes = in.classes;
   a.row_stride = in.row_stride;
   a.splits = static_cast<uint32_t>(splits);
@@ -712,7 +723,7 @@ __global__ __launch_bounds__(kLpThreads) void token_log_probs_bwd_kernel(const L
   const int64_t c0 = split * a.piece < a.classes ? split * a.piece : a.classes;
   const int64_t n = c0 + a.piece < a.classes ? a.piece : a.classes - c0;
   const int64_t base = row * a.row_stride + c0, out = row * a.classes + c0;
-  const int64_t head = ce_head(a.dz.p[0] + out, n), nvec = (n - head) / V;
+  const int64_t head = lp_head(a.dz.p[0] + out, n), nvec = (n - head) / V;
   if (y == a.ignore_index) {
     const Vec<T, V> zero{};
     for (int64_t j = threadIdx.x; j < nvec; j += kLpThreads)
@@ -728,8 +739,8 @@ __global__ __launch_bounds__(kLpThreads) void token_log_probs_bwd_kernel(const L
 #pragma unroll
   for (int k = 0; k <= K; ++k) {
     lse[k] = a.lse.p[k][row];
-    c[k] = a.cot_log_probs.p[0] != nullptr ? a.cot_log_probs.p[k][row] : A(0);
-    if (!valid) c[k] = __builtin_nan("");   // as the log probability of a token that is no class
+    // (NaN through the log probability of a token that is no class)
+    c[k] = a.cot_log_probs.p[0] == nullptr ? A(0) : valid ? a.cot_log_probs.p[k][row] : A(__builtin_nan(""));
     ch[k] = ENT ? a.cot_entropy.p[k][row] : A(0);
     none[k] = A(0);
     if (a.cot_top.p[0] != nullptr)
@@ -844,7 +855,7 @@ static int launch_log_probs_bwd_k(const LogProbBwdArgs& in) {
     if (in.cot_entropy != nullptr) a.cot_entropy.p[k] = static_cast<const A*>(in.cot_entropy[k]);
     if (in.cot_top_log_probs != nullptr && in.top > 0) a.cot_top.p[k] = static_cast<const A*>(in.cot_top_log_probs[k]);
   }
-  const int64_t splits = log_prob_splits(in.rows, in.classes, sizeof(T));
+  const int64_t splits = log_prob_splits(in.rows, in.classes, sizeof(T), true);
   a.classes = in.classes;
   a.row_stride = in.row_stride;
   a.splits = static_cast<uint32_t>(splits);

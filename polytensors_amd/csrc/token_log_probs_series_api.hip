@@ -1,18 +1,23 @@
 // C ABI of the token log-probability kernels.
+#include <algorithm>
+
 #include "token_log_probs_series.h"
 
 namespace pt {
 
-// Four blocks a compute unit, each with a 16-byte vector of every order a thread at least.
-int64_t log_prob_splits(int64_t rows, int64_t classes, int elem_size) {
-  const int64_t want = (1024 + rows - 1) / rows, most = classes / (256 * (16 / elem_size));
-  int64_t splits = want < most ? want : most;
-  if (splits > 64) splits = 64;
-  return splits < 1 ? 1 : splits;
+// Four blocks a compute unit, each with a 16-byte vector of every order a thread at least. Backward, where nothing has to be
+// joined, sixteen blocks where that leaves a thread as many vectors, so that the last round of blocks is short (1100 x
+// 128256 bfloat16, degree 2: 359 us with four, 328 so; forward 142 and 136, but 1500 x 50257 float32, degree 1, 98 and 114).
+int64_t log_prob_splits(int64_t rows, int64_t classes, int elem_size, bool backward) {
+  const int64_t round = 256 * (16 / elem_size);   // classes a block takes at a time
+  auto pieces = [&](int64_t blocks, int64_t least) { return std::min((blocks + rows - 1) / rows, classes / (round * least)); };
+  int64_t splits = pieces(1024, 1);
+  if (backward) splits = std::max(splits, pieces(4096, 16));
+  return std::max<int64_t>(1, std::min<int64_t>(64, splits));
 }
 
 size_t log_prob_workspace(int degree, int64_t rows, int64_t classes, int top, int elem_size) {
-  const int64_t splits = log_prob_splits(rows, classes, elem_size);
+  const int64_t splits = log_prob_splits(rows, classes, elem_size, false);
   if (splits == 1) return 0;
   const size_t acc = elem_size == 8 ? 8 : 4;
   return static_cast<size_t>(rows * splits) * (acc * (top + 3 * degree + 3) + sizeof(uint32_t) * top);

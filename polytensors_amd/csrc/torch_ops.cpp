@@ -1028,7 +1028,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_log_probs_series(const 
   Tensor workspace;
   if (wbytes > 0) workspace = at::empty({static_cast<int64_t>(wbytes)}, first.options().dtype(at::kByte));
   check_status(pt_token_log_probs_series_fwd(
-                   code, static_cast<int>(orders) - 1, cptrs(z).data(), rows, classes, rows ? first.stride(0) : classes,
+                   code, static_cast<int>(orders) - 1, cptrs(z).data(), rows, classes, rows > 1 ? first.stride(0) : classes,
                    tokens.data_ptr<int64_t>(), ignore_index, softcap, static_cast<int>(top), slices(log_probs).data(),
                    slices(entropy).data(), top_tokens.data_ptr<int64_t>(), slices(top_log_probs).data(),
                    slices(lse).data(), wbytes > 0 ? workspace.data_ptr() : nullptr, stream_of(first)),
@@ -1073,7 +1073,7 @@ Tensor token_log_probs_series_backward(const TensorList& z, const Tensor& tokens
   const bool tops = top > 0;
   check_status(pt_token_log_probs_series_bwd(
                    dtype_code(first.scalar_type()), static_cast<int>(orders) - 1, cptrs(z).data(), rows, classes,
-                   rows ? first.stride(0) : classes, tokens.data_ptr<int64_t>(), ignore_index, softcap,
+                   rows > 1 ? first.stride(0) : classes, tokens.data_ptr<int64_t>(), ignore_index, softcap,
                    static_cast<int>(top), tops ? top_tokens->data_ptr<int64_t>() : nullptr, lc.data(), ec.data(),
                    cot_log_probs.empty() ? nullptr : clp.data(), cot_entropy.empty() ? nullptr : cent.data(),
                    tops ? ctop.data() : nullptr, slices(out).data(), stream_of(first)),

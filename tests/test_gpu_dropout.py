@@ -132,6 +132,29 @@ def test_coefficient_gradients_and_their_derivative():
         assert torch.equal(second[k].cpu(), _want(2 * want, 10, 0.5))
 
 
+def test_wrapper_gradient_differentiates_again():
+    X, C = _series((6, 7), 1, 30, torch.float64), _series((6, 7), 1, 31, torch.float64)
+    x = PolyTensor(tuple(c.cuda() for c in X), requires_grad=True)
+    c = PolyTensor(tuple(t.cuda() for t in C), requires_grad=True)
+    with PolyTensor.plain_range(), PolyTensor.retain_wrappers():
+        y = PolyTensor.dropout(x, 0.5, seed=32)
+        (dx,) = torch.autograd.grad((y,), (x,), (c,), create_graph=True)
+        (dc,) = torch.autograd.grad((dx,), (c,), (PolyTensor(tuple(t.cuda() for t in X)),))
+        for k in range(2):
+            assert torch.equal(dx.coeffs[k].detach().cpu(), _want(C[k], 32, 0.5))
+            assert torch.equal(dc.coeffs[k].cpu(), _want(X[k], 32, 0.5))
+
+
+def test_a_seed_changed_before_the_gradient_is_an_error():
+    x = [torch.ones(8, device="cuda", requires_grad=True)]
+    seed = _seed(1)
+    with PolyTensor.plain_range(), PolyTensor.coefficient_autograd():
+        y = PolyTensor.dropout(PolyTensor(tuple(x)), 0.5, seed=seed)
+        seed.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y.coeffs[0].sum(), x[0])
+
+
 @pytest.mark.parametrize("recorded", [False, True])
 def test_complex_directions(recorded):
     X = _series((9, 8), 2, 12, torch.float32)

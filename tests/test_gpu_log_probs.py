@@ -228,6 +228,34 @@ def test_gradients_of_masked_padded_and_undefined_rows():
         assert (g[0, keep].double() - r[0]).abs().max() <= 2 * _bound(2, classes, dtype, r)
 
 
+def test_entropy_gradient_beside_a_token_that_is_no_class():
+    # the token has no part in the entropy: its gradient is finite, the log probability's is not
+    Z = _series((2, 300), 1, 28, torch.float64)
+    tokens = torch.tensor([300, 5])
+    z64 = [c.clone().requires_grad_() for c in Z]
+    ref = torch.autograd.grad(series64.log_probs(z64, torch.tensor([0, 5]))[1], z64, [torch.ones(2).double()] * 2)
+    leaves = [c.cuda().requires_grad_() for c in Z]
+    with PolyTensor.plain_range(), PolyTensor.coefficient_autograd():
+        y = PolyTensor.token_log_probs(PolyTensor(tuple(leaves)), tokens.cuda())
+    ones = [torch.ones(2, dtype=torch.float64, device="cuda")] * 2
+    _check_gradient(torch.autograd.grad(y.entropy.coeffs, leaves, ones, retain_graph=True), list(ref), 300, torch.float64)
+    assert torch.autograd.grad(y.log_probs.coeffs, leaves, ones)[0][0].isnan().all()
+
+
+def test_outputs_changed_in_place_before_the_gradient():
+    Z, tokens = _series((4, 200), 1, 29, torch.float64), _tokens(4, 200, 30)
+    results = []
+    for change in (False, True):
+        leaves = [c.cuda().requires_grad_() for c in Z]
+        with PolyTensor.plain_range(), PolyTensor.coefficient_autograd():
+            y = PolyTensor.token_log_probs(PolyTensor(tuple(leaves)), tokens.cuda(), top=2)
+        if change:
+            for c in (*y.log_probs.coeffs, *y.entropy.coeffs):
+                c.data.zero_()
+        results.append(torch.autograd.grad([*y.log_probs.coeffs, *y.entropy.coeffs], leaves, [torch.ones(4, dtype=torch.float64, device="cuda")] * 4))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 def test_gradient_against_differences():
     Z, tokens = _series((3, 40), 2, 17, torch.float64, 1.0), torch.tensor([3, 39, 0])
     cots = [_series((3,), 2, 18, torch.float64, 1.0), _series((3,), 2, 19, torch.float64, 1.0), _series((3, 2), 2, 20, torch.float64, 1.0)]
@@ -270,6 +298,10 @@ def test_leading_dimensions_strides_and_orders():
         wide = torch.randn(5, 200, device="cuda")
         part = PolyTensor.token_log_probs(PolyTensor._wrap((wide[:, 3:150],)), torch.arange(5, device="cuda"))
     assert one.log_probs.shape == () and abs(one.log_probs.value.item() - want[0][0][0].item()) <= _bound(2, 77, dtype, want[0][0])
+    column = torch.randn(60, 1, device="cuda")   # one row whose stride is below its length
+    with torch.no_grad(), PolyTensor.plain_range():
+        row = PolyTensor.token_log_probs(PolyTensor._wrap((column.t(),)), torch.tensor([7], device="cuda"))
+    _check(row.log_probs.coeffs, series64.log_probs([column.t().cpu().double()], torch.tensor([7]))[0], 60, dtype, "row")
     ref = series64.log_probs([wide[:, 3:150].cpu().double()], torch.arange(5))
     _check(part.log_probs.coeffs, ref[0], 147, dtype, "gap")
     # gradients through leading dimensions

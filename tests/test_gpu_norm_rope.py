@@ -285,6 +285,56 @@ def test_complex_directions():
     assert not yk.coeffs[1].is_complex()
 
 
+def test_complex_directions_in_reverse_mode():
+    # the gradient series along a complex direction: the real definition's, extended to complex coefficients
+    base, real, imag = _series((1, 2, 1, 16), 2, 3, torch.float64)
+    cot = _series((1, 1, 2, 16), 2, 4, torch.float64)
+    cos, sin = _tables(2, 16, torch.float64)
+    w = [c + (1.0 if i == 0 else 0.0) for i, c in enumerate(_series((16,), 2, 5, torch.float64, 0.2))]
+    x = [base, torch.complex(real, imag), torch.complex(imag, real)]
+    X, W = PolyTensor(tuple(c.cuda() for c in x), requires_grad=True), PolyTensor(tuple(c.cuda() for c in w), requires_grad=True)
+    key = PolyTensor(tuple(c.cuda() for c in (base, real, imag)))
+    with PolyTensor.plain_range(), PolyTensor.retain_wrappers():
+        y, _ = PolyTensor.qk_norm_rope(X, key, cos.cuda(), sin.cuda(), query_weight=W, eps=1e-3)
+        y.backward(_poly(cot))
+        # d/dx_0 of <cotangents, y> for real series is coefficient K of the gradient series; polynomial in the
+        # directions, so its value at complex ones comes from autograd over the complex definition
+        z = [c.to(torch.complex128).requires_grad_() for c in x]
+        v = [c.to(torch.complex128).requires_grad_() for c in w]
+        want = series64.norm_rope(z, v, cos, sin, torch.arange(2)[None], 1e-3, False)
+        total = sum((a * b).sum() for a, b in zip(want, cot[::-1]))
+        ref = torch.autograd.grad(total.real, z + v, retain_graph=True)
+        for i in range(3):   # (torch's gradient of the real part of a holomorphic function is the derivative's conjugate)
+            for got, r in ((X.grad, ref[2 - i].conj()), (W.grad, ref[5 - i].conj())):
+                got = got.coeffs[i].cpu().to(torch.complex128)
+                assert (got - (r.real if i == 0 else r)).abs().max() <= 1e-9 * max(1.0, r.abs().max().item()), i
+
+
+def test_gradients_of_nothing():
+    cos, sin = _tables(4, 16, torch.float32)
+    for B, L in ((0, 3), (2, 0)):
+        leaf = torch.empty(B, L, 2, 16, device="cuda", requires_grad=True)
+        w = torch.ones(16, device="cuda", requires_grad=True)
+        with PolyTensor.plain_range(), PolyTensor.coefficient_autograd():
+            x = PolyTensor((leaf,))
+            y, z = PolyTensor.qk_norm_rope(x, x, cos.cuda(), sin.cuda(), None, w, None)
+        dx, dw = torch.autograd.grad((y.value, z.value), (leaf, w), (torch.ones_like(y.value), torch.ones_like(z.value)))
+        assert dx.shape == leaf.shape and not dw.any()
+
+
+def test_another_stream():
+    q, k, w, cos, sin = _case(2, 40, 4, 2, 64, 64, 1, torch.float32)
+    stream = torch.cuda.Stream()
+    Q, K = _poly(q), _poly(k)
+    tables = cos.cuda(), sin.cuda()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream), torch.no_grad(), PolyTensor.plain_range():
+        y, _ = PolyTensor.qk_norm_rope(Q, K, *tables, eps=1e-5)
+    stream.synchronize()
+    _check(y.coeffs, series64.norm_rope(_double(q), None, cos.double(), sin.double(), torch.arange(40).expand(2, 40), 1e-5, False),
+           torch.float32)
+
+
 def test_captured_training_step():
     q, k, w, cos, sin = _case(2, 9, 4, 2, 64, 64, 2, torch.bfloat16)
     leaves = [c.cuda().requires_grad_() for c in (*q, *k, w[0][0], w[1][0])]
