@@ -38,7 +38,7 @@ def why_ineligible(logits, tokens, top, softcap, ignore_index, allow_grad=False)
         return reason
     if logits.ndim < 1 or logits.shape[-1] == 0:
         return "logits must be (..., C) with at least one class"
-    if logits.dtype not in _DTYPES or any(_gate.real_dtype(c.dtype) != logits.dtype for c in logits.coeffs):
+    if logits.dtype not in _DTYPES or _gate.real_dtype(logits.coeffs[-1].dtype) != logits.dtype:   # (the higher orders share one)
         return "logits must be float16/bfloat16/float32/float64 in every order"
     if logits.shape[-1] >= 2 ** 31 or logits.numel() // logits.shape[-1] >= 2 ** 31:
         return "more than 2^31 - 1 rows or classes"
@@ -57,6 +57,11 @@ def why_ineligible(logits, tokens, top, softcap, ignore_index, allow_grad=False)
     return None
 
 
+def _series(stacked):
+    """The series of a coefficient-stacked result of the operator (disjoint real orders: no checks)."""
+    return PolyTensor._wrap(stacked.unbind(0))
+
+
 class _SeriesLogProbs(torch.autograd.Function):
     """Log probabilities, entropy and (with ``top``) the alternatives' log probabilities of (N, C) logits with
     their gradient series, under wrapper-level autograd."""
@@ -69,8 +74,8 @@ class _SeriesLogProbs(torch.autograd.Function):
         ctx.save_for_backward(logits, tokens, lse, entropy, top_tokens)
         ctx.meta = (ignore_index, softcap)
         ctx.mark_non_differentiable(top_tokens)
-        outputs = tuple(PolyTensor.from_stacked(y) for y in (log_probs, entropy.clone()))
-        return (*outputs, top_tokens, PolyTensor.from_stacked(top_log_probs)) if top else outputs
+        outputs = (_series(log_probs), _series(entropy.clone()))   # (the entropy is saved: a caller may change its own)
+        return (*outputs, top_tokens, _series(top_log_probs)) if top else outputs
 
     @staticmethod
     def backward(ctx, *gradients):
@@ -90,7 +95,7 @@ class _SeriesLogProbs(torch.autograd.Function):
             return None, None, None, None, None
         dz = _ops.token_log_probs_series_backward(_rows(logits.coeffs), tokens, ignore_index, softcap, lse, entropy,
                                                   top_tokens, *cots)
-        return PolyTensor.from_stacked(dz), None, None, None, None
+        return _series(dz), None, None, None, None
 
 
 def _run(logits, tokens, ignore_index, softcap, top):
@@ -99,8 +104,8 @@ def _run(logits, tokens, ignore_index, softcap, top):
         return _SeriesLogProbs.apply(logits, tokens, ignore_index, softcap, top)
     log_probs, entropy, top_tokens, top_log_probs, _ = _ops.token_log_probs_series(_rows(logits.coeffs), tokens, ignore_index,
                                                                                    softcap, top)
-    outputs = tuple(map(PolyTensor.from_stacked, (log_probs, entropy)))
-    return (*outputs, top_tokens, PolyTensor.from_stacked(top_log_probs)) if top else outputs
+    outputs = (_series(log_probs), _series(entropy))
+    return (*outputs, top_tokens, _series(top_log_probs)) if top else outputs
 
 
 def _complex_run(logits, tokens, ignore_index, softcap, top):

@@ -26,14 +26,14 @@ def why_ineligible(query, key, cos, sin, positions, query_weight, key_weight, ep
     reason = _gate.common_reason(operands, allow_plain_grad=_gate.wrapper_grad(*operands), complex_ok=True)
     if reason is not None:
         return reason
-    dtype, device = _gate.real_dtype(query.dtype), query.device
+    dtype, device = query.dtype, query.device   # (a series' dtype is its constant order's, real here)
     if dtype not in _DTYPES:
-        return f"dtype {query.dtype} is not supported (float32, float64, bfloat16 or float16)"
+        return f"dtype {dtype} is not supported (float32, float64, bfloat16 or float16)"
     acc = torch.float64 if dtype == torch.float64 else torch.float32
     grads = torch.is_grad_enabled()
     for x in operands:   # (a series' higher orders share one dtype: its last order stands for them)
         series = isinstance(x, PolyTensor)
-        if x.dtype != dtype or (series and _gate.real_dtype(x.coeffs[-1].dtype) != dtype):
+        if x.dtype != dtype or (series and x.coeffs[-1].dtype != dtype and _gate.real_dtype(x.coeffs[-1].dtype) != dtype):
             return "query, key and the weights must share one dtype"
         if x.device != device:
             return "operands and weights must be on one device"
@@ -73,8 +73,8 @@ def why_ineligible(query, key, cos, sin, positions, query_weight, key_weight, ep
 
 def _heads(coeffs):
     """Coefficients with one common set of strides and a head's elements side by side (else copies)."""
-    first = coeffs[0]
-    if (first.shape[-1] <= 1 or first.stride(-1) == 1) and all(c.stride() == first.stride() for c in coeffs):
+    strides = coeffs[0].stride()
+    if (strides[-1] == 1 or coeffs[0].shape[-1] <= 1) and all(c.stride() == strides for c in coeffs[1:]):
         return list(coeffs)
     return [c.contiguous() for c in coeffs]
 
@@ -120,12 +120,15 @@ class _SeriesNormRope(torch.autograd.Function):
 
 def _run(query, key, query_weight, key_weight, cos, sin, positions, eps, interleaved):
     """The operation on real series or ordinary tensors of one kind (key None: queries alone)."""
-    if _gate.wrapper_grad(query, key, query_weight, key_weight):
-        return _SeriesNormRope.apply(query, key, query_weight, key_weight, cos, sin, positions, eps, interleaved)
+    recorded = False
+    if torch.is_grad_enabled():
+        if _gate.wrapper_grad(query, key, query_weight, key_weight):
+            return _SeriesNormRope.apply(query, key, query_weight, key_weight, cos, sin, positions, eps, interleaved)
+        recorded = _gate.coefficient_graph(query, key, query_weight, key_weight)
     series = isinstance(query, PolyTensor)
     q, k = _heads(_gate.coefficients(query, 0)), [] if key is None else _heads(_gate.coefficients(key, 0))
     args = (q, k, cos, sin, positions, _weight(query_weight), _weight(key_weight), eps, interleaved)
-    if _gate.coefficient_graph(query, key, query_weight, key_weight):
+    if recorded:
         out = _ops.norm_rope_series_orders(*args)
         parts = [out[:len(q)], out[len(q):]]
     else:
