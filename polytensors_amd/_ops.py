@@ -8,7 +8,8 @@ the K+1 coefficient tensors of a series as a ``Tensor[]`` (the reference's tuple
 storage, passed without stacking copies) and returns one coefficient-stacked
 tensor ``[K+1, ...]``; on any other device the dispatcher raises. This module
 adds what belongs in Python: the fake (shape) implementations and the
-coefficient-level autograd of every operator. Outputs never alias inputs.
+coefficient-level autograd of the operators (that of the norm and rotation, of the
+token log probabilities and of dropout is recorded in C++). Outputs never alias inputs.
 """
 
 import math

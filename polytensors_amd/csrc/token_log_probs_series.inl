@@ -22,6 +22,11 @@
 // finds one class after the other in passes over the row.
 //
 // Few rows are cut into pieces, a block each, whose states and alternatives a second kernel joins.
+//
+// HBM bounds long rows: 8192 x 32000 float32 at degree 4 with 5 alternatives 803 us, 6.5 TB/s; 4096 x 32001 bfloat16 at degree
+// 3 170 us, 6.2 TB/s, its gradient 419 us, 5.0 TB/s (streams over the same buffers 158 and 340). 16-bit logits of low
+// degree come nearer the vector units' rate: 2048 x 128256 bfloat16, degree 1, 20 alternatives 223 us, 4.7 TB/s.
+// Few rows are bound by a block's chain of loads and barriers, about 10 us, and the join's 7 (8 x 131072: 9.5 + 7.0).
 #pragma once
 
 #include <type_traits>
